@@ -1,7 +1,9 @@
 /*
  * rgd_b200.h — C ABI of librgd_b200.so: hand-written sm_100a CUDA kernels for the
  * rgd_triton operator set (row L2 / RMS norms, per-head LayerNorm, rotary
- * embedding, fused LayerNorm+rotary, FlashAttention with additive bias).
+ * embedding, fused LayerNorm+rotary, FlashAttention with additive bias) and
+ * for what surrounds it when tokens are generated one by one: a paged
+ * key-value cache, attention over it, a learned relative position bias.
  *
  * Conventions
  *   - Every pointer is a DEVICE pointer on the current device.  The caller owns
@@ -10,14 +12,15 @@
  *   - Sizes are int64_t; dtype codes are RGD_F32 / RGD_F16 / RGD_BF16.
  *   - `stream` is a cudaStream_t passed as void* (NULL = legacy default stream).
  *   - Return value: 0 success; <0 argument error (see RGD_E_*); >=1000 is
- *     1000 + cudaError_t; RGD_E_TIMEOUT a bounded device-side wait that ran out.
+ *     1000 + cudaError_t; RGD_E_TIMEOUT a bounded device-side wait that ran out,
+ *     RGD_E_PAGE a bad page-table entry (both by rgd_device_status alone).
  *     Argument errors correspond to the AssertionError / RuntimeError the
  *     reference's host wrappers raise; the Python layer re-raises them as such.
  *   - All entry points are re-entrant.  Process-wide state: a memo of the
  *     per-kernel cudaFuncSetAttribute opt-ins for large shared memory and of
  *     occupancy queries (each made once per device and kernel), the launch
- *     counter, the sticky status word of the bounded device-side waits, and the
- *     fixed scratch of rgd_rmsnorm_bwd_static.
+ *     counter, the sticky status words of the bounded device-side waits and of
+ *     the paged cache, and the fixed scratch of rgd_rmsnorm_bwd_static.
  *
  * Each declaration cites the reference interface (file:line inside the
  * rgd_triton project) whose launch it replaces.
@@ -47,6 +50,8 @@ extern "C" {
 #define RGD_E_DEVICE       -7   /* current device is not compute capability 10.x        */
 #define RGD_E_BIAS_SHAPE   -8   /* bias is neither (1,Tk) "vector" nor (Tq,Tk) "matrix" */
 #define RGD_E_TIMEOUT    2001   /* bounded device-side wait expired                     */
+#define RGD_E_PAGE       2002   /* a length, position or page-table entry (all read on
+                                   the device) was outside the cache or the table       */
 #define RGD_E_CUDA_BASE  1000   /* 1000 + cudaError_t                                   */
 
 /* ---- tensor views ------------------------------------------------------ */
@@ -77,10 +82,12 @@ const char *rgd_status_string(int status);
 int         rgd_abi_version(void);
 /* Number of kernels this library has launched in the calling process. */
 int64_t     rgd_launch_count(void);
-/* Sticky status of the tensor-memory kernels' bounded device-side waits:
- * RGD_OK, or RGD_E_TIMEOUT if a wait ran out since the last call (the flag is
- * cleared by the call).  Synchronises the device; meant for tests, smoke
- * checks and debugging, not for the per-step path. */
+/* Sticky status of what only the device sees: RGD_OK; RGD_E_TIMEOUT if a bounded
+ * wait of the tensor-memory kernels ran out since the last call; RGD_E_PAGE if a
+ * paged-cache call met a length, position or page-table entry out of range.  The
+ * reported flag is cleared by the call (with both set, the next call reports the
+ * other).  Synchronises the device; meant for tests, smoke checks and debugging,
+ * not for the per-step path. */
 int         rgd_device_status(void);
 
 /* Test hook for the bounded device-side waits (no counterpart in the
@@ -355,6 +362,109 @@ int rgd_attn_bwd_uses_tmem(const rgd_heads *q, const rgd_heads *k,
                            const rgd_heads *dk, const rgd_heads *dv, int64_t B,
                            int64_t H, int64_t Tq, int64_t Tk, int64_t d,
                            int dtype);
+
+/* ---- learned relative position bias ------------------------------------- */
+/* bias[h, i, j] = weight[bucket(j - i - offset), h].  With side = num_buckets
+ * (or num_buckets / 2 when bidirectional), a distance n >= 0 falls into the
+ * bucket k < side with borders[k - 1] <= n < borders[k]: `borders` is a HOST
+ * array of side - 1 non-decreasing positive distances (read during the call).
+ * Bidirectional: n = |j - i - offset|, and keys after the query (j > i +
+ * offset) use the upper half of the buckets; else n = max(i + offset - j, 0). */
+#define RGD_RELBIAS_MAX_SIDE 256
+typedef struct rgd_relbias {
+    const void    *weight;          /* (num_buckets, H)                        */
+    int64_t        stride_bucket;
+    int64_t        stride_head;
+    int            dtype;           /* RGD_F32 / RGD_F16 / RGD_BF16             */
+    int            num_buckets;
+    int            bidirectional;
+    const int32_t *borders;
+} rgd_relbias;
+
+/* out: [H, Tq, Tk] through element strides, unit key stride, base and strides
+ * multiples of 16 bytes (rows of any Tk, e.g. padded ones).  One rounding to
+ * out_dtype.  The bias matrix of rgd_attn_fwd. */
+int rgd_relbias_fwd(const rgd_relbias *bias, void *out, int64_t stride_h,
+                    int64_t stride_q, int64_t H, int64_t Tq, int64_t Tk,
+                    int64_t offset, int out_dtype, void *stream);
+/* Scratch bytes of rgd_relbias_bwd. */
+int64_t rgd_relbias_bwd_workspace_bytes(int64_t H, int64_t Tq, int64_t Tk,
+                                        int num_buckets);
+/* dweight[k, h] = sum of dbias[h, i, j] over bucket(j - i - offset) = k, in a
+ * fixed order, rounded once to bias->dtype.  dbias: [H, Tq, Tk] of dtype
+ * through element strides (any, 0 included), unit key stride.  dweight: dense
+ * [num_buckets, H].  bias->weight and its strides are not used. */
+int rgd_relbias_bwd(const rgd_relbias *bias, const void *dbias,
+                    int64_t stride_h, int64_t stride_q, int dtype,
+                    void *dweight, int64_t H, int64_t Tq, int64_t Tk,
+                    int64_t offset, void *workspace, int64_t workspace_bytes,
+                    void *stream);
+
+/* ---- paged key-value cache ------------------------------------------------ */
+/* Keys and values of many sequences in pages of page_size tokens.  The cache
+ * tensors are (page, slot, head, channel) views, channel stride 1, any strides
+ * otherwise.  Position p of sequence b lies in page page_table[b, p / page_size],
+ * slot p % page_size.  `page_table` and `lengths` are read on the device when
+ * the call runs; what they hold out of range (a negative length, a position
+ * past max_pages * page_size, a page outside [0, num_pages)) is never followed
+ * and is reported by rgd_device_status() as RGD_E_PAGE.  Table entries past a
+ * sequence's last page are not read. */
+typedef struct rgd_paged {
+    void          *k;
+    void          *v;
+    int64_t        k_stride_p, k_stride_s, k_stride_h;
+    int64_t        v_stride_p, v_stride_s, v_stride_h;
+    int64_t        num_pages;
+    int64_t        page_size;
+    const int32_t *page_table;      /* [B, max_pages] */
+    int64_t        table_stride;    /* elements from one sequence to the next */
+    int64_t        max_pages;
+    const int32_t *lengths;         /* [B] */
+} rgd_paged;
+
+/* Where position `position` of the sequence with the table row `row` lies:
+ * element offsets of its head 0 from cache->k and cache->v.  The rule of the
+ * kernels, evaluated on the host: cache->page_table must be readable there.
+ * RGD_E_PAGE for what the kernels would not follow. */
+int rgd_paged_slot(const rgd_paged *cache, int64_t row, int64_t position,
+                   int64_t *k_offset, int64_t *v_offset);
+
+/* Appends the first counts[b] (N when counts is NULL) of N new tokens to each of
+ * B sequences that hold lengths[b] tokens: key and value, (B, Hkv, N, d) views,
+ * go to positions lengths[b] + i.  With `pos` ([2, P, R], sin and cos, element
+ * strides; R even, R <= d) the first R channels of key are rotated as
+ * interleaved pairs by the angles of their position on the way, and so is
+ * `query` (B, Hq, N, d; may be NULL) into query_out; rows of query past counts[b]
+ * are copied.  fp32 arithmetic, one rounding.  A token whose position is not in
+ * the cache or not below P is not written.  Two tokens of one call that map to
+ * the same slot leave either's values there, channel by channel.  dtype RGD_F16
+ * / RGD_BF16, pos_dtype any, d <= 128. */
+int rgd_paged_append(const rgd_heads *key, const rgd_heads *value,
+                     const rgd_heads *query, const rgd_heads *query_out,
+                     const rgd_paged *cache, const int32_t *counts,
+                     const void *pos, int64_t pos_stride_s,
+                     int64_t pos_stride_n, int64_t P, int64_t R, int64_t B,
+                     int64_t N, int64_t Hq, int64_t Hkv, int64_t d, int dtype,
+                     int pos_dtype, void *stream);
+
+/* Scratch bytes of rgd_paged_attn for this problem on the current device. */
+int64_t rgd_paged_attn_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv,
+                                       int64_t d, int64_t max_pages,
+                                       int64_t page_size);
+/* Attention of one token per sequence over its cached keys and values:
+ * o = softmax(q k^T * scale + bias) v over positions [0, lengths[b]) (lengths
+ * count the token itself, whose position is lengths[b] - 1).  q, o: (B, Hq, 1,
+ * d) views; query head h reads cache head h / (Hq / Hkv).  `bias` (NULL: none)
+ * adds weight[bucket(lengths[b] - 1 - j), h].  lse (NULL or fp32 [B, Hq]):
+ * log-sum-exp.  A sequence of length 0 gets zeros and lse -inf; so does one
+ * without a usable page.  Keys of pages out of range are left out.  dtype
+ * RGD_F16 / RGD_BF16, d <= 128, Hq a multiple of Hkv.  The order of all sums
+ * depends on the lengths and the device alone, not on the run. */
+int rgd_paged_attn(const rgd_heads *q, const rgd_paged *cache,
+                   const rgd_relbias *bias, const rgd_heads *o, float *lse,
+                   int64_t B, int64_t Hq, int64_t Hkv, int64_t d,
+                   float softmax_scale, int dtype, void *workspace,
+                   int64_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

@@ -8,7 +8,8 @@ entries; ``rgd_triton_b200.compat.install()`` registers both under the
 from . import ops, functional  # noqa: F401
 from .ops import (  # noqa: F401
     CachableModule, FlashAttention, L2Normalize, FusedL2Normalize2, FusedHeadLayerNorm,
-    FusedRMSNorm, FusedRMSNorm2, RoPE, FusedLNRoPE,
+    FusedRMSNorm, FusedRMSNorm2, RoPE, FusedLNRoPE, RelativePositionBias, PagedCacheAppend,
+    PagedAttention,
 )
 
 __version__ = "0.1.0"

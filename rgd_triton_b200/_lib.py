@@ -21,7 +21,7 @@ RGD_BIAS_NONE, RGD_BIAS_VECTOR, RGD_BIAS_MATRIX = 0, 1, 2
 
 RGD_E_INVALID, RGD_E_DTYPE, RGD_E_SIZE, RGD_E_STRIDE = -1, -2, -3, -4
 RGD_E_NULL, RGD_E_WORKSPACE, RGD_E_DEVICE, RGD_E_BIAS_SHAPE = -5, -6, -7, -8
-RGD_E_TIMEOUT = 2001
+RGD_E_TIMEOUT, RGD_E_PAGE = 2001, 2002
 
 DTYPE_CODE = {torch.float32: RGD_F32, torch.float16: RGD_F16, torch.bfloat16: RGD_BF16}
 
@@ -42,8 +42,23 @@ class Bias(C.Structure):
                 ("kind", C.c_int), ("dtype", C.c_int), ("tiles", C.c_void_p)]
 
 
+class RelBias(C.Structure):
+    """rgd_relbias: weights of a relative position bias; borders is a host array."""
+    _fields_ = [("weight", C.c_void_p), ("stride_bucket", C.c_int64), ("stride_head", C.c_int64), ("dtype", C.c_int),
+                ("num_buckets", C.c_int), ("bidirectional", C.c_int), ("borders", C.POINTER(C.c_int32))]
+
+
+class Paged(C.Structure):
+    """rgd_paged: (page, slot, head, channel) views of the cached keys and values, page table and lengths."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_stride_p", C.c_int64), ("k_stride_s", C.c_int64),
+                ("k_stride_h", C.c_int64), ("v_stride_p", C.c_int64), ("v_stride_s", C.c_int64), ("v_stride_h", C.c_int64),
+                ("num_pages", C.c_int64), ("page_size", C.c_int64), ("page_table", C.c_void_p), ("table_stride", C.c_int64),
+                ("max_pages", C.c_int64), ("lengths", C.c_void_p)]
+
+
 _i64, _i32, _f32, _vp = C.c_int64, C.c_int, C.c_float, C.c_void_p
 _pRows, _pHeads, _pBias = C.POINTER(Rows), C.POINTER(Heads), C.POINTER(Bias)
+_pRelBias, _pPaged = C.POINTER(RelBias), C.POINTER(Paged)
 _pi64, _pi32, _pvp = C.POINTER(C.c_int64), C.POINTER(C.c_int), C.POINTER(C.c_void_p)
 
 # name -> (restype, argtypes); must list every function of include/rgd_b200.h.
@@ -85,6 +100,13 @@ SIGNATURES = {
     "rgd_attn_bias_tiles_build": (_i32, [_pBias, _i64, _i64, _i64, _i64, _f32, _vp, _i64, _vp]),
     "rgd_attn_fwd_uses_tmem": (_i32, [_pHeads] * 4 + [_i64] * 5 + [_f32, _i32]),
     "rgd_attn_bwd_uses_tmem": (_i32, [_pHeads] * 8 + [_i64] * 5 + [_i32]),
+    "rgd_relbias_fwd": (_i32, [_pRelBias, _vp] + [_i64] * 6 + [_i32, _vp]),
+    "rgd_relbias_bwd_workspace_bytes": (_i64, [_i64] * 3 + [_i32]),
+    "rgd_relbias_bwd": (_i32, [_pRelBias, _vp, _i64, _i64, _i32, _vp] + [_i64] * 4 + [_vp, _i64, _vp]),
+    "rgd_paged_slot": (_i32, [_pPaged, _i64, _i64, _pi64, _pi64]),
+    "rgd_paged_append": (_i32, [_pHeads] * 4 + [_pPaged, _vp, _vp] + [_i64] * 9 + [_i32, _i32, _vp]),
+    "rgd_paged_attn_workspace_bytes": (_i64, [_i64] * 6),
+    "rgd_paged_attn": (_i32, [_pHeads, _pPaged, _pRelBias, _pHeads, _vp] + [_i64] * 4 + [_f32, _i32, _vp, _i64, _vp]),
 }
 
 _lib = None

@@ -86,7 +86,7 @@ int cached_occupancy(const void *kernel, int threads, size_t smem) {
 
 }  // namespace rgd
 
-extern "C" int rgd_abi_version(void) { return 3; }
+extern "C" int rgd_abi_version(void) { return 4; }
 
 extern "C" int64_t rgd_launch_count(void) { return rgd::g_launches.load(std::memory_order_relaxed); }
 
@@ -112,6 +112,7 @@ extern "C" const char *rgd_status_string(int status) {
         case RGD_E_DEVICE: return "device is not compute capability 10.x (sm_100)";
         case RGD_E_BIAS_SHAPE: return "Last 2 dimensions of bias must be (1, seqlen_k) or (seqlen_q, seqlen_k)";
         case RGD_E_TIMEOUT: return "bounded device-side wait expired";
+        case RGD_E_PAGE: return "length, position or page-table entry outside the paged cache";
     }
     if (status >= RGD_E_CUDA_BASE && status < RGD_E_TIMEOUT)
         return cudaGetErrorString((cudaError_t)(status - RGD_E_CUDA_BASE));

@@ -21,6 +21,9 @@ int64_t tmem_bwd_workspace_bytes(int64_t B, int64_t H, int64_t Tq);
 int build_bias_tiles(const void *bias, int64_t sb, int64_t sh, int64_t sq, int64_t Bb, int64_t Hb, int64_t Tq, int64_t Tk,
                      int dtype, float thr, void *tiles, cudaStream_t st);
 }  // namespace attn
+namespace paged {
+int status_fetch();
+}  // namespace paged
 }  // namespace rgd
 
 using namespace rgd;
@@ -112,7 +115,10 @@ extern "C" int64_t rgd_attn_lse_rows(int64_t Tq) { return Tq < 0 ? RGD_E_INVALID
 extern "C" int rgd_device_status(void) {
     const int v = attn::tmem_status_fetch();
     if (v < 0) return RGD_E_CUDA_BASE;
-    return v == 0 ? RGD_OK : RGD_E_TIMEOUT;
+    if (v != 0) return RGD_E_TIMEOUT;
+    const int page = paged::status_fetch();
+    if (page < 0) return RGD_E_CUDA_BASE;
+    return page == 0 ? RGD_OK : RGD_E_PAGE;
 }
 
 extern "C" int rgd_attn_fwd(const rgd_heads *q, const rgd_heads *k, const rgd_heads *v, const rgd_bias *bias,

@@ -133,6 +133,27 @@ __device__ __forceinline__ float warp_group_sum(float v, int width) {
 
 static inline bool is_aligned(const void *p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 
+// ---------------------------------------------------------------------------
+// Fast division of a 31-bit unsigned value by a runtime constant
+// (q = umulhi(n, mul) >> shr), precomputed on the host.
+// ---------------------------------------------------------------------------
+struct FastDiv {
+    uint32_t mul, shr, div;
+};
+__host__ __device__ __forceinline__ uint32_t fdiv(uint32_t n, const FastDiv &f) {
+    return f.div == 1 ? n : ((uint32_t)(((uint64_t)n * f.mul) >> 32) >> f.shr);
+}
+static inline FastDiv make_fastdiv(uint32_t d) {
+    FastDiv f{0, 0, d};
+    if (d <= 1) return f;
+    uint32_t lg = 0;
+    while ((1ull << lg) < d) ++lg;                 // ceil(log2 d)
+    const uint32_t pw = 31 + lg;
+    f.mul = (uint32_t)(((1ull << pw) + d - 1) / d);
+    f.shr = pw - 32;
+    return f;
+}
+
 static inline int64_t ceil_div64(int64_t a, int64_t b) { return (a + b - 1) / b; }
 static inline int next_pow2(int v) {
     int p = 1;

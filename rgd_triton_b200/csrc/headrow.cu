@@ -33,12 +33,6 @@ struct HeadTensor {
     int64_t rows;       // B * D1 * D2
 };
 
-// Fast division of a 31-bit unsigned value by a runtime constant
-// (q = umulhi(n, mul) >> shr), precomputed on the host.
-struct FastDiv {
-    uint32_t mul, shr, div;
-};
-
 struct HeadParams {
     HeadTensor t[2];
     int64_t split;      // tiles that belong to tensor 0
@@ -72,10 +66,6 @@ __device__ __forceinline__ void load_table(const TP *row, int col, int R, bool v
 #pragma unroll
         for (int e = 0; e < VE; ++e) out[e] = (col + e < R) ? to_f32<TP>(row[col + e]) : 0.f;
     }
-}
-
-__device__ __forceinline__ uint32_t fdiv(uint32_t n, const FastDiv &f) {
-    return f.div == 1 ? n : (__umulhi(n, f.mul) >> f.shr);
 }
 
 // Row id -> (batch, outer, inner) indices of a head tensor.
@@ -703,17 +693,6 @@ struct HeadCall {
 bool heads_vec_ok(const rgd_heads &v, int esize) {
     const int ve = 16 / esize;
     return is_aligned(v.ptr, 16) && v.stride_b % ve == 0 && v.stride_h % ve == 0 && v.stride_n % ve == 0;
-}
-
-FastDiv make_fastdiv(uint32_t d) {
-    FastDiv f{0, 0, d};
-    if (d <= 1) return f;
-    uint32_t lg = 0;
-    while ((1ull << lg) < d) ++lg;                 // ceil(log2 d)
-    const uint32_t pw = 31 + lg;
-    f.mul = (uint32_t)(((1ull << pw) + d - 1) / d);
-    f.shr = pw - 32;
-    return f;
 }
 
 template <typename T, typename TP, int VPT, int OP>

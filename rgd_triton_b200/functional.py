@@ -17,6 +17,9 @@ entry point here             reference entry it replaces
 ``flash_attn_func``          flash_attn/flash_attn_triton_cached.py:1131-1133
 ===========================  =======================================================
 
+and, beyond the reference, what a model needs around them to generate token by token and to train
+with a position bias: ``relative_position_bias_fn``, ``paged_cache_append_fn``, ``paged_attention_func``.
+
 Differences from the reference, all deliberate:
 
 * the entry points run on the native host path (``csrc/host/torch_host.cpp``: checks, allocation,
@@ -41,6 +44,7 @@ survive ``python -O``.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
 import os
 import threading
@@ -49,7 +53,7 @@ import weakref
 import torch
 
 from . import _lib
-from ._lib import Bias, Heads, Rows
+from ._lib import Bias, Heads, Paged, RelBias, Rows
 
 _FLOATS = (torch.float16, torch.bfloat16, torch.float32)
 
@@ -1052,4 +1056,277 @@ def flash_attn_func(q, k, v, bias=None, causal=False, softmax_scale=None, return
         o, lse = FlashAttnFunc.apply(q, k, v, bias, causal, softmax_scale, kernel_cache)
     if large:
         o = o.contiguous()      # as the native path and the padded head dims return it
+    return (o, lse) if return_lse else o
+
+
+# --------------------------------------------------------------------------
+# Learned relative position bias
+# --------------------------------------------------------------------------
+@functools.lru_cache(maxsize=None)
+def relative_position_borders(side: int, max_distance: int) -> tuple:
+    """The least distance of each of the buckets 1 .. side - 1 of one direction: the first half of the buckets hold
+    one distance each, bucket half + j begins where (n / half)^(side - half) >= (max_distance / half)^j, the last one
+    holds everything further.  In whole numbers: a rounded logarithm puts distances that lie on a border (16, 32 and
+    64 with 16 buckets up to 128) on either side of it."""
+    half = side // 2
+    rest = side - half
+    found = list(range(1, half + 1))
+    for j in range(1, rest):
+        reached = lambda n: n ** rest >= half ** (rest - j) * max_distance ** j
+        n = max(half, round(half * (max_distance / half) ** (j / rest)))
+        while not reached(n):
+            n += 1
+        while n > half and reached(n - 1):
+            n -= 1
+        found.append(n)
+    return tuple(found)
+
+
+def _check_relbias(weight, bidirectional: bool, max_distance: int) -> int:
+    """The number of buckets of one direction."""
+    _require(weight.ndim == 2, f"weight must be (num_buckets, nheads), got {tuple(weight.shape)}")
+    _require(weight.dtype in _FLOATS, "Only support fp16, bf16, and fp32")
+    buckets = weight.shape[0]
+    _require(not bidirectional or buckets % 2 == 0, "bidirectional buckets come in two halves: their number must be even")
+    side = buckets // 2 if bidirectional else buckets
+    _require(2 <= side <= 256, f"2 to 256 buckets in each direction, got {side}")
+    _require(side // 2 < max_distance < 1 << 28, f"max_distance must be above {side // 2}, the distances with a bucket of their own")
+    _lib.require_device(weight)
+    return side
+
+
+def _relbias_struct(weight, bidirectional: bool, max_distance: int, side: int) -> RelBias:
+    borders = relative_position_borders(side, max_distance)
+    return RelBias(weight.data_ptr(), weight.stride(0), weight.stride(1), _lib.dtype_code(weight.dtype), weight.shape[0],
+                   1 if bidirectional else 0, (C.c_int32 * len(borders))(*borders))
+
+
+def _bias_rows(seqlen_q: int, seqlen_k: int, nheads: int, dtype, device):
+    """(1, nheads, seqlen_q, seqlen_k) whose rows begin on 16 bytes, as the attention kernels stage them."""
+    full = torch.empty((1, nheads, seqlen_q, (seqlen_k + 7) // 8 * 8), dtype=dtype, device=device)
+    return full[..., :seqlen_k]
+
+
+def _relbias_forward(weight, seqlen_q, seqlen_k, bidirectional, max_distance, offset, dtype):
+    side = _check_relbias(weight, bidirectional, max_distance)
+    _require(dtype in _FLOATS, "Only support fp16, bf16, and fp32")
+    _require(seqlen_q >= 0 and seqlen_k >= 0, "sequence lengths must not be negative")
+    out = _bias_rows(seqlen_q, seqlen_k, weight.shape[1], dtype, weight.device)
+    s = _relbias_struct(weight, bidirectional, max_distance, side)
+    with _lib.device_guard(weight):
+        code = _lib.load().rgd_relbias_fwd(C.byref(s), out.data_ptr(), out.stride(1), out.stride(2), weight.shape[1], seqlen_q,
+                                           seqlen_k, offset, _lib.dtype_code(dtype), _lib.stream_ptr())
+    if code:
+        _lib.check(code, "relbias_fwd")
+    return out
+
+
+def _relbias_backward(dbias, buckets, wdtype, bidirectional, max_distance, offset):
+    dbias = _last_contig(dbias)
+    _, nheads, seqlen_q, seqlen_k = dbias.shape
+    dweight = torch.empty((buckets, nheads), dtype=wdtype, device=dbias.device)
+    side = _check_relbias(dweight, bidirectional, max_distance)
+    lib = _lib.load()
+    nbytes = int(lib.rgd_relbias_bwd_workspace_bytes(nheads, seqlen_q, seqlen_k, buckets))
+    _require(nbytes >= 0, "relbias_bwd: bad sizes")
+    s = _relbias_struct(dweight, bidirectional, max_distance, side)
+    with _lib.device_guard(dbias):
+        work = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dbias.device)
+        code = lib.rgd_relbias_bwd(C.byref(s), dbias.data_ptr(), dbias.stride(1), dbias.stride(2), _lib.dtype_code(dbias.dtype),
+                                   dweight.data_ptr(), nheads, seqlen_q, seqlen_k, offset, work.data_ptr(), work.numel(),
+                                   _lib.stream_ptr())
+    if code:
+        _lib.check(code, "relbias_bwd")
+    return dweight
+
+
+class RelativePositionBiasFunc(torch.autograd.Function):
+    """weight[bucket(j - i - offset)] as a (1, nheads, seqlen_q, seqlen_k) bias; the gradient sums the bias's over
+    each bucket's positions, in a fixed order."""
+
+    @staticmethod
+    def forward(ctx, weight, seqlen_q, seqlen_k, bidirectional, max_distance, offset, dtype):
+        ctx.args = weight.shape[0], weight.dtype, bidirectional, max_distance, offset
+        return _relbias_forward(weight, seqlen_q, seqlen_k, bidirectional, max_distance, offset, dtype)
+
+    @staticmethod
+    def backward(ctx, dbias):
+        return _relbias_backward(dbias, *ctx.args), None, None, None, None, None, None
+
+
+def relative_position_bias_fn(weight, seqlen_q, seqlen_k, bidirectional=True, max_distance=128, offset=0, dtype=None):
+    """A learned bias by the distance between query and key, (1, nheads, seqlen_q, seqlen_k) in ``dtype`` (default:
+    the weight's), for ``flash_attn_func``'s ``bias``.
+
+    weight: (num_buckets, nheads).  Query i stands at position i + offset, key j at j.  Distances below half a
+    direction's buckets have one each, further ones share them in even steps of the logarithm up to ``max_distance``,
+    the last bucket holds what is beyond.  ``bidirectional``: the upper half of the buckets is for keys after the query;
+    otherwise those count as distance 0.  Differentiable in weight (sums in fp32 or more, bit-reproducible).  The rows
+    of the result begin on 16 bytes whatever seqlen_k is (it may be a view of a wider tensor)."""
+    seqlen_q, seqlen_k, offset, max_distance = int(seqlen_q), int(seqlen_k), int(offset), int(max_distance)
+    bidirectional, dtype = bool(bidirectional), dtype or weight.dtype
+    if not _needs_grad(weight):
+        return _relbias_forward(weight, seqlen_q, seqlen_k, bidirectional, max_distance, offset, dtype)
+    return RelativePositionBiasFunc.apply(weight, seqlen_q, seqlen_k, bidirectional, max_distance, offset, dtype)
+
+
+# --------------------------------------------------------------------------
+# Paged key-value cache
+# --------------------------------------------------------------------------
+def _check_paged(k_cache, v_cache, page_table, lengths, batch: int, like, nheads_k: int) -> None:
+    d = like.shape[-1]
+    for c, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
+        _require(c.ndim == 4, f"{name} must be (pages, page_size, nheads, headdim), got {tuple(c.shape)}")
+        _require(c.dtype == like.dtype, f"{name} must have the tokens' type {like.dtype}, got {c.dtype}")
+        _require(c.shape[2:] == (nheads_k, d), f"{name} holds {tuple(c.shape[2:])} heads and channels, not {(nheads_k, d)}")
+        _require(c.stride(-1) == 1 or d <= 1 or c.numel() == 0, f"{name}: last dimension must be contiguous")
+        _require(c.device == like.device, f"{name} is on another device")
+    _require(k_cache.shape[:2] == v_cache.shape[:2], "k_cache and v_cache must have the same pages")
+    _require(k_cache.shape[1] >= 1, "pages must hold at least one token")
+    _require(page_table.ndim == 2 and page_table.shape[0] == batch, f"page_table must be ({batch}, max_pages), got {tuple(page_table.shape)}")
+    _require(lengths.ndim == 1 and lengths.shape[0] == batch, f"lengths must be ({batch},), got {tuple(lengths.shape)}")
+    _check_ints(like, page_table=page_table, lengths=lengths)
+
+
+def _check_ints(like, **tensors) -> None:
+    for name, t in tensors.items():
+        _require(t.dtype == torch.int32, f"{name} must be int32, got {t.dtype}")
+        _require(t.device == like.device, f"{name} is on another device")
+
+
+def _paged_struct(k_cache, v_cache, page_table, lengths) -> Paged:
+    return Paged(k_cache.data_ptr(), v_cache.data_ptr(), *k_cache.stride()[:3], *v_cache.stride()[:3], k_cache.shape[0],
+                 k_cache.shape[1], page_table.data_ptr(), page_table.stride(0), page_table.shape[1], lengths.data_ptr())
+
+
+def _refuse_grad(what: str, *tensors) -> None:
+    _require(not _needs_grad(*tensors), f"{what} has no backward pass: call it under torch.no_grad()")
+
+
+def _written(*caches) -> None:
+    """Tells autograd that these were written in place."""
+    for c in caches:
+        if not c.is_inference():
+            torch.autograd.graph.increment_version(c)
+
+
+def _append_launch(key, value, k_cache, v_cache, page_table, lengths, pos_emb, query, counts):
+    _require(key.ndim == 4, f"key must be (batch, seqlen, nheads, headdim), got {tuple(key.shape)}")
+    batch, n, nheads_k, d = key.shape
+    _require(value.shape == key.shape, f"value shape {tuple(value.shape)} does not match key")
+    _require(key.dtype in (torch.float16, torch.bfloat16), "Only support fp16 and bf16")
+    _require(d <= 128, "Only supports head dimensions up to 128")
+    _require(query is None or pos_emb is not None, "a query is only rotated: pass pos_emb with it")
+    tokens = [key, value] + ([] if query is None else [query])
+    if query is not None:
+        _require(query.ndim == 4 and query.shape[:2] == (batch, n) and query.shape[3] == d,
+                 f"query must be ({batch}, {n}, nheads, {d}), got {tuple(query.shape)}")
+    _require(all(t.dtype == key.dtype for t in tokens), "All tensors must have the same type")
+    _require(all(t.device == key.device for t in tokens), "All tensors must be on the same device")
+    _check_paged(k_cache, v_cache, page_table, lengths, batch, key, nheads_k)
+    for c, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
+        _require(all(s > 0 for s, size in zip(c.stride(), c.shape) if size > 1), f"{name} is written: its slots must not share memory")
+    if counts is not None:
+        _require(counts.ndim == 1 and counts.shape[0] == batch, f"counts must be ({batch},), got {tuple(counts.shape)}")
+        _check_ints(key, counts=counts)
+    P = R = 0
+    if pos_emb is not None:
+        _require(pos_emb.ndim == 3 and pos_emb.shape[0] == 2, "pos_emb must be [2, P, R]: sin and cos")
+        _require(pos_emb.dtype in _FLOATS, "Only support fp16, bf16, and fp32")
+        _require(pos_emb.device == key.device, "pos_emb must be on the tensors' device")
+        P, R = pos_emb.shape[1:]
+        _require(R % 2 == 0 and R <= d, f"pos_emb must rotate an even number of channels, at most {d}, got {R}")
+    _lib.require_device(key)
+    key, value, lengths = _last_contig(key), _last_contig(value), lengths.contiguous()
+    page_table = _last_contig(page_table)
+    query_out = None
+    if query is not None:
+        query = _last_contig(query)
+        query_out = torch.empty_like(query)
+    if counts is not None:
+        counts = counts.contiguous()
+    if pos_emb is not None:
+        pos_emb = _last_contig(pos_emb)
+    heads = lambda t: None if t is None else C.byref(_attn_heads(t))
+    cache = _paged_struct(k_cache, v_cache, page_table, lengths)
+    with _lib.device_guard(key):
+        code = _lib.load().rgd_paged_append(
+            heads(key), heads(value), heads(query), heads(query_out), C.byref(cache), None if counts is None else counts.data_ptr(),
+            None if pos_emb is None else pos_emb.data_ptr(), 0 if pos_emb is None else pos_emb.stride(0),
+            0 if pos_emb is None else pos_emb.stride(1), P, R, batch, n, 0 if query is None else query.shape[2], nheads_k, d,
+            _lib.dtype_code(key.dtype), _lib.RGD_F32 if pos_emb is None else _lib.dtype_code(pos_emb.dtype), _lib.stream_ptr())
+    if code:
+        _lib.check(code, "paged_append")
+    return query_out
+
+
+def paged_cache_append_fn(key, value, k_cache, v_cache, page_table, lengths, pos_emb=None, query=None, counts=None):
+    """Append new tokens to a paged key-value cache, rotating keys (and queries) by their position on the way.
+
+    key, value: (batch, n, nheads_k, headdim), n new tokens of each sequence; k_cache, v_cache: (pages, page_size,
+    nheads_k, headdim), written in place, any strides with a unit channel stride (a cache kept head by head is passed
+    as its transpose(1, 2)); page_table: (batch, max_pages) int32, the page of each page_size positions of a sequence;
+    lengths: (batch,) int32, the tokens that each sequence holds so far.  Token i of sequence b goes to position
+    lengths[b] + i.  ``counts``: (batch,) int32, only the first counts[b] tokens are new ones (default: all n).
+    ``pos_emb``: [2, P, R], sin and cos as for RoPE; the first R channels of key are rotated in fp32 and rounded once.
+    ``query``: (batch, n, nheads, headdim), returned rotated by the same positions; tokens past counts[b] are copied.
+
+    Returns the rotated query, or None without one.  lengths is not changed.  Nothing is read back from the device:
+    a token whose position has no page, or no row in pos_emb, is left out, and
+    ``rgd_triton_b200._lib.load().rgd_device_status()`` reports it.  No two tokens of a call may map to the same slot.
+    No backward pass."""
+    _refuse_grad("paged_cache_append", key, value, query, k_cache, v_cache, pos_emb)
+    out = _append_launch(key, value, k_cache, v_cache, page_table, lengths, pos_emb, query, counts)
+    _written(k_cache, v_cache)
+    return out
+
+
+def _paged_attn_launch(q, k_cache, v_cache, page_table, lengths, softmax_scale, rel_weight, bidirectional, max_distance):
+    _require(q.ndim == 4 and q.shape[1] == 1, f"q must be (batch, 1, nheads, headdim), got {tuple(q.shape)}")
+    batch, _, nheads, d = q.shape
+    _require(q.dtype in (torch.float16, torch.bfloat16), "Only support fp16 and bf16")
+    _require(d <= 128, "FlashAttention only support head dimensions up to 128")
+    nheads_k = k_cache.shape[2] if k_cache.ndim == 4 else 0
+    _require(nheads == 0 or (nheads_k > 0 and nheads % nheads_k == 0), f"{nheads} query heads do not share {nheads_k} key heads evenly")
+    _check_paged(k_cache, v_cache, page_table, lengths, batch, q, nheads_k)
+    bias = None
+    if rel_weight is not None:
+        _require(rel_weight.ndim == 2 and rel_weight.shape[1] == nheads, f"rel_weight must be (num_buckets, {nheads})")
+        _require(rel_weight.device == q.device, "rel_weight is on another device")
+        side = _check_relbias(rel_weight, bidirectional, max_distance)
+        bias = C.byref(_relbias_struct(rel_weight, bidirectional, max_distance, side))
+    _lib.require_device(q)
+    q, lengths, page_table = _last_contig(q), lengths.contiguous(), _last_contig(page_table)
+    lib = _lib.load()
+    cache = _paged_struct(k_cache, v_cache, page_table, lengths)
+    with _lib.device_guard(q):
+        o = torch.empty_like(q)
+        lse = torch.empty((batch, nheads), device=q.device, dtype=torch.float32)
+        nbytes = int(lib.rgd_paged_attn_workspace_bytes(batch, nheads, nheads_k, d, page_table.shape[1], k_cache.shape[1]))
+        _require(nbytes >= 0, "paged_attn: bad sizes")
+        work = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=q.device)
+        code = lib.rgd_paged_attn(C.byref(_attn_heads(q)), C.byref(cache), bias, C.byref(_attn_heads(o)), lse.data_ptr(), batch, nheads,
+                                  nheads_k, d, float(softmax_scale), _lib.dtype_code(q.dtype), work.data_ptr(), work.numel(),
+                                  _lib.stream_ptr())
+    if code:
+        _lib.check(code, "paged_attn")
+    return o, lse
+
+
+def paged_attention_func(q, k_cache, v_cache, page_table, lengths, softmax_scale=None, rel_weight=None, bidirectional=False,
+                         max_distance=128, return_lse=False):
+    """Attention of one new token per sequence over its cached keys and values.
+
+    q: (batch, 1, nheads, headdim); k_cache, v_cache, page_table as for ``paged_cache_append_fn``, nheads a multiple of
+    their heads (query head h reads cache head h // (nheads // nheads_k)); lengths: (batch,) int32, the tokens to attend
+    to, the new one included (after an append: the lengths before it plus 1).  A sequence of length 0 gets zeros.
+    ``rel_weight``: (num_buckets, nheads), adds ``relative_position_bias_fn``'s bias for the query position
+    lengths[b] - 1, in fp32 (``bidirectional`` and ``max_distance`` as there).  Returns o like q, and with
+    ``return_lse`` the (batch, nheads) log-sum-exp.
+
+    Nothing is read back from the device: keys of pages outside the pool are left out, a length past the table's pages
+    is cut there, and ``rgd_triton_b200._lib.load().rgd_device_status()`` reports both.  No backward pass."""
+    _refuse_grad("paged_attention", q, k_cache, v_cache, rel_weight)
+    scale = 1.0 / math.sqrt(max(q.shape[-1], 1)) if softmax_scale is None else softmax_scale
+    o, lse = _paged_attn_launch(q, k_cache, v_cache, page_table, lengths, scale, rel_weight, bool(bidirectional), int(max_distance))
     return (o, lse) if return_lse else o

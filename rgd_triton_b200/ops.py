@@ -2,9 +2,10 @@
 ``rgd_triton/ops.py`` (lines 12-249) with the same class names, constructor and
 ``forward`` signatures, defaults, parameter names (``weight``, ``weight1``,
 ``weight2``) and ``enable_cache`` / ``.cache`` behaviour, backed by the sm_100a
-CUDA library instead of Triton kernels.
+CUDA library instead of Triton kernels; and, beyond the reference, ``RelativePositionBias``,
+``PagedCacheAppend`` and ``PagedAttention``.
 
-``state_dict`` s interchange with the reference: only the two RMSNorm modules
+``state_dict`` s interchange with the reference: of its modules only the two RMSNorm ones
 own parameters, under the same names and initialised to ones.
 """
 from __future__ import annotations
@@ -230,7 +231,54 @@ class FusedLNRoPE(CachableModule):
                         norm_eps=eps, kernel_cache=self.cache)
 
 
+class RelativePositionBias(nn.Module):
+    """Learned bias by the distance between query and key, (1, nheads, Tq, Tk), for ``FlashAttention``'s ``bias``;
+    ``weight`` is (num_buckets, nheads).  The buckets are described at ``functional.relative_position_bias_fn``."""
+
+    def __init__(self, num_buckets, nheads, max_distance=128, bidirectional=True, device=None, dtype=None):
+        super().__init__()
+        side = num_buckets // 2 if bidirectional else num_buckets
+        if bidirectional and num_buckets % 2 != 0:
+            raise AssertionError("bidirectional buckets come in two halves: their number must be even")
+        if not 2 <= side <= 256:
+            raise AssertionError(f"2 to 256 buckets in each direction, got {side}")
+        if not side // 2 < max_distance < 1 << 28:
+            raise AssertionError(f"max_distance must be above {side // 2}, the distances with a bucket of their own")
+        self.num_buckets, self.nheads = num_buckets, nheads
+        self.max_distance, self.bidirectional = max_distance, bidirectional
+        self.weight = nn.Parameter(torch.empty((num_buckets, nheads), device=device, dtype=dtype))
+        self.reset_parameters()
+
+    def reset_parameters(self) -> None:
+        nn.init.normal_(self.weight, std=0.02)
+
+    def forward(self, seqlen_q, seqlen_k, offset=0, dtype=None):
+        return F_.relative_position_bias_fn(self.weight, seqlen_q, seqlen_k, self.bidirectional, self.max_distance, offset, dtype)
+
+    def extra_repr(self) -> str:
+        return f"{self.num_buckets}, {self.nheads}, max_distance={self.max_distance}, bidirectional={self.bidirectional}"
+
+
+class PagedCacheAppend(nn.Module):
+    """Appends new keys and values to a paged cache, in place, rotating keys (and the query, which is returned) by
+    their position: ``functional.paged_cache_append_fn``."""
+
+    def forward(self, key, value, k_cache, v_cache, page_table, lengths, pos_emb=None, query=None, counts=None):
+        return F_.paged_cache_append_fn(key, value, k_cache, v_cache, page_table, lengths, pos_emb, query, counts)
+
+
+class PagedAttention(nn.Module):
+    """Attention of one new token per sequence, q (B, 1, h, d), over a paged cache:
+    ``functional.paged_attention_func``.  ``rel_bias``: a RelativePositionBias whose bias is added."""
+
+    def forward(self, q, k_cache, v_cache, page_table, lengths, softmax_scale=None, rel_bias=None):
+        if rel_bias is None:
+            return F_.paged_attention_func(q, k_cache, v_cache, page_table, lengths, softmax_scale)
+        return F_.paged_attention_func(q, k_cache, v_cache, page_table, lengths, softmax_scale, rel_bias.weight,
+                                       rel_bias.bidirectional, rel_bias.max_distance)
+
+
 __all__ = [
     "CachableModule", "FlashAttention", "L2Normalize", "FusedL2Normalize2", "FusedHeadLayerNorm",
-    "FusedRMSNorm", "FusedRMSNorm2", "RoPE", "FusedLNRoPE",
+    "FusedRMSNorm", "FusedRMSNorm2", "RoPE", "FusedLNRoPE", "RelativePositionBias", "PagedCacheAppend", "PagedAttention",
 ]
