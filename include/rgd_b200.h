@@ -383,7 +383,8 @@ typedef struct rgd_relbias {
 
 /* out: [H, Tq, Tk] through element strides, unit key stride, base and strides
  * multiples of 16 bytes (rows of any Tk, e.g. padded ones).  One rounding to
- * out_dtype.  The bias matrix of rgd_attn_fwd. */
+ * out_dtype.  The bias matrix of rgd_attn_fwd.  Tq <= 2^22, Tk <= 2^28, Tq * Tk
+ * <= 2^44, |offset| <= 2^29. */
 int rgd_relbias_fwd(const rgd_relbias *bias, void *out, int64_t stride_h,
                     int64_t stride_q, int64_t H, int64_t Tq, int64_t Tk,
                     int64_t offset, int out_dtype, void *stream);

@@ -1,8 +1,18 @@
 // Learned relative position bias: bias[h, i, j] = w[bucket(j - i - offset), h], and the gradient of w.
 //
-// The matrix depends on j - i alone: H rows of Tq + Tk - 1 values, written H Tq Tk times.  The gradient is the
-// sum over the diagonals, then over the diagonals of each bucket.
+// Forward.  The matrix depends on j - i alone, so every row of a tile of it is a window of one short row of values:
+// row i of the tile is that row shifted by one element more than row i + 1.  A CTA evaluates the short row once, keeps
+// it in shared memory at each of the shifts that a 16-byte address can have, and lets the copy engine write the rows
+// from there (one bulk store each): no thread touches an element of the output but those past the last 16 bytes of a
+// row.  Bound by writing H Tq Tk elements.
+//
+// Gradient.  dw[k] is a sum over whole diagonals.  The matrix is taken in blocks of 8 x 8; a thread walks down blocks
+// (I, J), (I + 1, J + 1), ..., whose 15 diagonals are the same ones, and keeps their sums in registers, so an element
+// costs one addition.  The threads of a warp have neighbouring J and read 512 consecutive bytes of a row together.
+// The diagonal sums of a warp then go to the buckets, which are ranges of diagonals, in an order that is fixed by the
+// sizes: the result is the same every time.  Bound by reading H Tq Tk elements.
 #include "relbias.cuh"
+#include "sm100_prims.cuh"
 
 namespace rgd {
 namespace relbias {
@@ -15,63 +25,216 @@ struct FwdParams {
     void *out;
     int64_t o_sh, o_sq;
     int Tq, Tk, offset;
+    int rows, cols;             // of a tile; both multiples of 8
 };
 
-constexpr int THREADS = 256;
+constexpr int FWD_THREADS = 256;
+constexpr int FWD_COLS = 2048;
+
+// Shared memory: the short row (tile cols + rows values, rounded up) at each shift, the borders, the head's weights.
+template <typename T> __host__ __device__ constexpr int fwd_row_values(int rows, int cols) { return rows + cols + 16 / (int)sizeof(T); }
+template <typename T> constexpr size_t fwd_smem(int rows, int cols, int buckets) {
+    return 16 * (size_t)fwd_row_values<T>(rows, cols) + MAX_SIDE * sizeof(int) + (size_t)buckets * sizeof(T);
+}
 
 template <typename T>
-__global__ void __launch_bounds__(THREADS) relbias_fwd_kernel(const __grid_constant__ FwdParams p) {
-    const int h = blockIdx.y;
-    const int64_t n = (int64_t)p.Tq * p.Tk;
-    T *out = reinterpret_cast<T *>(p.out) + (int64_t)h * p.o_sh;
-    for (int64_t e = (int64_t)blockIdx.x * THREADS + threadIdx.x; e < n; e += (int64_t)gridDim.x * THREADS) {
-        const int i = (int)(e / p.Tk), j = (int)(e - (int64_t)i * p.Tk);
-        const int k = bucket_of(p.borders.at, p.borders.side, p.borders.both, j - i - p.offset);
-        out[(int64_t)i * p.o_sq + j] = from_f32<T>(load_as_f32(p.w, k * p.w_sk + h * p.w_sh, p.w_dtype));
+__global__ void __launch_bounds__(FWD_THREADS) relbias_fwd_kernel(const __grid_constant__ FwdParams p) {
+    constexpr int SHIFTS = 16 / sizeof(T);
+    using V = Vec<T, SHIFTS>;
+    extern __shared__ __align__(16) unsigned char raw[];
+    const int L = fwd_row_values<T>(p.rows, p.cols);
+    T *lut = reinterpret_cast<T *>(raw);                // [SHIFTS][L]: lut[s][x] = row[x + s]
+    int *at = reinterpret_cast<int *>(raw + 16 * (size_t)L);
+    T *w = reinterpret_cast<T *>(at + MAX_SIDE);
+    const int h = blockIdx.z, i0 = blockIdx.y * p.rows, j0 = blockIdx.x * p.cols, tid = threadIdx.x;
+    const int side = p.borders.side, both = p.borders.both;
+    for (int k = tid; k < side - 1; k += FWD_THREADS) at[k] = p.borders.at[k];
+    for (int k = tid; k < side * (1 + both); k += FWD_THREADS) w[k] = from_f32<T>(load_as_f32(p.w, k * p.w_sk + h * p.w_sh, p.w_dtype));
+    __syncthreads();
+    // row[x] belongs to j - i = (j0 - i0) - (rows - 1) + x: row r of the tile begins at x = rows - 1 - r
+    const int first = j0 - i0 - (p.rows - 1) - p.offset;
+    for (int x = tid; x < L; x += FWD_THREADS) lut[x] = w[bucket_of(at, side, both, first + x)];
+    __syncthreads();
+    for (int x = tid * SHIFTS; x + SHIFTS < L; x += FWD_THREADS * SHIFTS) {
+        const V a = load_vec<T, SHIFTS>(lut + x), b = load_vec<T, SHIFTS>(lut + x + SHIFTS);
+#pragma unroll
+        for (int s = 1; s < SHIFTS; ++s) {
+            V c;
+#pragma unroll
+            for (int e = 0; e < SHIFTS; ++e) c.v[e] = e + s < SHIFTS ? a.v[(e + s) % SHIFTS] : b.v[(e + s) % SHIFTS];
+            store_vec<T, SHIFTS>(lut + s * L + x, c);
+        }
     }
+    sm100::fence_proxy_async_smem();
+    __syncthreads();
+    const int rows = min(p.rows, p.Tq - i0), cols = min(p.cols, p.Tk - j0), even = cols / SHIFTS * SHIFTS;
+    T *out = reinterpret_cast<T *>(p.out) + (int64_t)h * p.o_sh + (int64_t)i0 * p.o_sq + j0;
+    for (int r = tid; r < rows; r += FWD_THREADS) {
+        const int x = p.rows - 1 - r, s = x % SHIFTS;
+        if (even > 0) sm100::bulk_store_1d(out + (int64_t)r * p.o_sq, lut + s * L + (x - s), (uint32_t)(even * sizeof(T)));
+        for (int j = even; j < cols; ++j) out[(int64_t)r * p.o_sq + j] = lut[x + j];
+    }
+    sm100::bulk_commit();
+    sm100::bulk_wait_read();
 }
 
 struct BwdParams {
     Borders borders;
     const void *g;
     int64_t g_sh, g_sq;
-    int g_dtype;
     void *dw;
     int w_dtype;
-    double *sums;               // [H, Tq + Tk - 1]
+    float *parts;               // [H][CTAs of a head][buckets]
     int H, Tq, Tk, offset;
+    int chunk;                  // 8-row blocks of a CTA
+    int across;                 // CTAs side by side
 };
 
-// One thread per diagonal.
-__global__ void __launch_bounds__(THREADS) relbias_diagonals_kernel(const __grid_constant__ BwdParams p) {
-    const int h = blockIdx.y, e = blockIdx.x * THREADS + threadIdx.x;
-    if (e >= p.Tq + p.Tk - 1) return;
-    const int difference = e - (p.Tq - 1);
-    double sum = 0.;
-    for (int i = max(0, -difference); i < p.Tq && i + difference < p.Tk; ++i)
-        sum += load_as_f32(p.g, h * p.g_sh + i * p.g_sq + i + difference, p.g_dtype);
-    p.sums[(int64_t)h * (p.Tq + p.Tk - 1) + e] = sum;
+constexpr int BWD_WARPS = 4, BWD_THREADS = BWD_WARPS * 32;
+constexpr int DIAGS = 32 * 8 + 7;       // of a warp's 32 neighbouring block diagonals
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(BWD_THREADS) relbias_bwd_kernel(const __grid_constant__ BwdParams p) {
+    __shared__ float diag[BWD_WARPS][DIAGS + 1];
+    extern __shared__ float hist[];                     // [BWD_WARPS][buckets]
+    __shared__ int at[MAX_SIDE];
+    sm100::grid_trigger();
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, h = blockIdx.y;
+    const int side = p.borders.side, both = p.borders.both, buckets = side * (1 + both);
+    const int row_chunk = blockIdx.x / p.across, m = blockIdx.x - row_chunk * p.across;
+    const int I0 = row_chunk * p.chunk, nI = (p.Tq + 7) / 8, nJ = (p.Tk + 7) / 8;
+    const int k_warp = m * BWD_THREADS - (I0 + p.chunk - 1) + warp * 32, k = k_warp + lane;       // J - I
+    for (int x = tid; x < side - 1; x += BWD_THREADS) at[x] = p.borders.at[x];
+    for (int x = tid; x < BWD_WARPS * buckets; x += BWD_THREADS) hist[x] = 0.f;
+
+    float acc[15];
+#pragma unroll
+    for (int e = 0; e < 15; ++e) acc[e] = 0.f;
+    const T *g = reinterpret_cast<const T *>(p.g) + (int64_t)h * p.g_sh;
+    const int I1 = min(I0 + p.chunk, nI);
+    for (int I = max(I0, -k); I < I1 && I + k < nJ; ++I) {
+        const int i = I * 8, j = (I + k) * 8;
+        const T *at0 = g + (int64_t)i * p.g_sq + j;
+        if (VEC && j + 8 <= p.Tk && i + 8 <= p.Tq) {
+            constexpr int PER = 16 / sizeof(T);
+            Vec<T, PER> x[8][8 / PER];
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+#pragma unroll
+                for (int c = 0; c < 8 / PER; ++c) x[r][c] = load_vec_stream<T, PER>(at0 + r * p.g_sq + c * PER);
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+#pragma unroll
+                for (int c = 0; c < 8; ++c) acc[c - r + 7] += to_f32<T>(x[r][c / PER].v[c % PER]);
+        } else {
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+#pragma unroll
+                for (int c = 0; c < 8; ++c)
+                    if (i + r < p.Tq && j + c < p.Tk) acc[c - r + 7] += to_f32<T>(at0[r * p.g_sq + c]);
+        }
+    }
+    __syncthreads();
+    // the warp's diagonals: j - i = 8 k_warp - 7 + index; neighbouring threads share seven of them
+#pragma unroll
+    for (int e = 0; e < 8; ++e) diag[warp][lane * 8 + e] = acc[e];
+    if (lane == 31)
+#pragma unroll
+        for (int e = 8; e < 15; ++e) diag[warp][lane * 8 + e] = acc[e];
+    __syncwarp();
+    if (lane < 31)
+#pragma unroll
+        for (int e = 8; e < 15; ++e) diag[warp][lane * 8 + e] += acc[e];
+    __syncwarp();
+    const int lo = 8 * k_warp - 7 - p.offset, hi = lo + DIAGS - 1;
+    float *mine = hist + warp * buckets;
+    const int from = bucket_of(at, side, both, lo), to = bucket_of(at, side, both, hi);
+    for (int b = 0; b < buckets; ++b) {
+        // bucket b holds the differences [d0, d1]
+        if (from == to && b != from) continue;          // the whole window is in one bucket
+        const int s = b < side ? b : b - side;
+        const int near = s == 0 ? 0 : at[s - 1], far = s == side - 1 ? 1 << 30 : at[s] - 1;
+        int d0, d1;
+        if (b < side) {
+            d0 = -far;
+            d1 = s == 0 && !both ? 1 << 30 : -near;
+        } else {
+            d0 = max(near, 1);
+            d1 = far;
+        }
+        d0 = max(d0, lo);
+        d1 = min(d1, hi);
+        if (d0 > d1) continue;
+        float sum = 0.f;
+        for (int d = d0 + lane; d <= d1; d += 32) sum += diag[warp][d - lo];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane == 0) mine[b] = sum;
+    }
+    __syncthreads();
+    float *out = p.parts + ((int64_t)h * gridDim.x + blockIdx.x) * buckets;
+    for (int b = tid; b < buckets; b += BWD_THREADS)
+        out[b] = (hist[b] + hist[buckets + b]) + (hist[2 * buckets + b] + hist[3 * buckets + b]);
 }
 
-// One CTA per (bucket, head).
-__global__ void __launch_bounds__(THREADS) relbias_buckets_kernel(const __grid_constant__ BwdParams p) {
-    __shared__ double part[THREADS];
-    const int k = blockIdx.x, h = blockIdx.y, n = p.Tq + p.Tk - 1;
+// Adds the CTAs' parts, in 64 bits: one CTA per (bucket, head).
+__global__ void __launch_bounds__(BWD_THREADS) relbias_sum_kernel(const __grid_constant__ BwdParams p, int parts) {
+    __shared__ double warp_sum[BWD_WARPS];
+    sm100::grid_wait();
+    const int b = blockIdx.x, h = blockIdx.y, buckets = gridDim.x;
     double sum = 0.;
-    for (int e = threadIdx.x; e < n; e += THREADS)
-        if (bucket_of(p.borders.at, p.borders.side, p.borders.both, e - (p.Tq - 1) - p.offset) == k) sum += p.sums[(int64_t)h * n + e];
-    part[threadIdx.x] = sum;
-    for (int o = THREADS / 2; o > 0; o >>= 1) {
-        __syncthreads();
-        if ((int)threadIdx.x < o) part[threadIdx.x] += part[threadIdx.x + o];
-    }
-    if (threadIdx.x == 0) store_from_f32(p.dw, (int64_t)k * p.H + h, p.w_dtype, (float)part[0]);
+    for (int c = threadIdx.x; c < parts; c += BWD_THREADS) sum += p.parts[((int64_t)h * parts + c) * buckets + b];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if ((threadIdx.x & 31) == 0) warp_sum[threadIdx.x >> 5] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0)
+        store_from_f32(p.dw, (int64_t)b * p.H + h, p.w_dtype, (float)((warp_sum[0] + warp_sum[1]) + (warp_sum[2] + warp_sum[3])));
+}
+
+// Rows of a CTA: few for small problems, so that they spread over the chip.
+struct BwdGrid {
+    int chunk, across, ctas;
+};
+BwdGrid bwd_grid(int64_t H, int64_t Tq, int64_t Tk) {
+    const int64_t nI = (Tq + 7) / 8, nJ = (Tk + 7) / 8;
+    int chunk = 32;
+    auto across = [&] { return ceil_div64(nJ + chunk - 1, BWD_THREADS); };
+    auto ctas = [&] { return ceil_div64(nI, chunk) * across(); };
+    while (chunk > 4 && H * ctas() < 8 * num_sms()) chunk /= 2;
+    return {chunk, (int)across(), (int)ctas()};
+}
+
+template <typename T>
+int launch_fwd(FwdParams &p, int H, cudaStream_t st) {
+    // Tiles of 128 rows spread the evaluation of the short row over 128 of its windows; problems that would not fill
+    // the chip with them take 32.
+    p.cols = (int)(p.Tk < FWD_COLS ? (p.Tk + 7) / 8 * 8 : FWD_COLS);
+    const int64_t across = ceil_div64(p.Tk, p.cols);
+    p.rows = across * ceil_div64(p.Tq, 128) * H >= 2 * num_sms() ? 128 : 32;
+    const size_t smem = fwd_smem<T>(p.rows, p.cols, p.borders.side * (1 + p.borders.both));
+    static_assert(fwd_smem<T>(128, FWD_COLS, 2 * MAX_SIDE) <= 48 << 10, "more than a kernel gets without asking");
+    relbias_fwd_kernel<T><<<dim3((unsigned)across, (unsigned)ceil_div64(p.Tq, p.rows), (unsigned)H), FWD_THREADS, smem, st>>>(p);
+    count_launch();
+    return check_launch();
+}
+template <typename T>
+int launch_bwd(const BwdParams &p, const BwdGrid &grid, bool vec, cudaStream_t st) {
+    const int buckets = p.borders.side * (1 + p.borders.both);
+    const size_t smem = (size_t)BWD_WARPS * buckets * sizeof(float);
+    auto kernel = vec ? relbias_bwd_kernel<T, true> : relbias_bwd_kernel<T, false>;
+    kernel<<<dim3((unsigned)grid.ctas, (unsigned)p.H), BWD_THREADS, smem, st>>>(p);
+    count_launch();
+    if (int e = check_launch()) return e;
+    return sm100::launch_pdl(relbias_sum_kernel, dim3((unsigned)buckets, (unsigned)p.H), BWD_THREADS, 0, st, p, grid.ctas);
 }
 
 int check_sizes(int64_t H, int64_t Tq, int64_t Tk, int64_t offset) {
     if (H < 0 || Tq < 0 || Tk < 0) return RGD_E_INVALID;
-    // differences of positions are 32-bit
-    if (H > 65535 || Tq > (1 << 28) || Tk > (1 << 28) || offset > (1 << 29) || offset < -(1 << 29)) return RGD_E_SIZE;
+    // differences of positions are 32-bit, and so are the grids
+    if (H > 65535 || Tq > (1 << 22) || Tk > (1 << 28) || offset > (1 << 29) || offset < -(1 << 29) ||
+        Tq * Tk > 1ll << 44)
+        return RGD_E_SIZE;
     return RGD_OK;
 }
 
@@ -94,20 +257,16 @@ extern "C" int rgd_relbias_fwd(const rgd_relbias *bias, void *out, int64_t strid
     p.w = bias->weight; p.w_sk = bias->stride_bucket; p.w_sh = bias->stride_head; p.w_dtype = bias->dtype;
     p.out = out; p.o_sh = stride_h; p.o_sq = stride_q;
     p.Tq = (int)Tq; p.Tk = (int)Tk; p.offset = (int)offset;
-    const int64_t blocks = ceil_div64(Tq * Tk, relbias::THREADS);
-    const dim3 grid((unsigned)(blocks < 4096 ? blocks : 4096), (unsigned)H);
     cudaStream_t st = (cudaStream_t)stream;
-    if (out_dtype == RGD_F32) relbias::relbias_fwd_kernel<float><<<grid, relbias::THREADS, 0, st>>>(p);
-    else if (out_dtype == RGD_F16) relbias::relbias_fwd_kernel<__half><<<grid, relbias::THREADS, 0, st>>>(p);
-    else relbias::relbias_fwd_kernel<__nv_bfloat16><<<grid, relbias::THREADS, 0, st>>>(p);
-    count_launch();
-    return check_launch();
+    if (out_dtype == RGD_F32) return relbias::launch_fwd<float>(p, (int)H, st);
+    return out_dtype == RGD_F16 ? relbias::launch_fwd<__half>(p, (int)H, st) : relbias::launch_fwd<__nv_bfloat16>(p, (int)H, st);
 }
 
 extern "C" int64_t rgd_relbias_bwd_workspace_bytes(int64_t H, int64_t Tq, int64_t Tk, int num_buckets) {
-    (void)num_buckets;
     if (int e = relbias::check_sizes(H, Tq, Tk, 0)) return e;
-    return H * (Tq + Tk) * (int64_t)sizeof(double);
+    if (num_buckets < 1) return RGD_E_INVALID;
+    if (H == 0 || Tq == 0 || Tk == 0) return 0;
+    return H * relbias::bwd_grid(H, Tq, Tk).ctas * (int64_t)num_buckets * (int64_t)sizeof(float);
 }
 
 extern "C" int rgd_relbias_bwd(const rgd_relbias *bias, const void *dbias, int64_t stride_h, int64_t stride_q, int dtype, void *dweight,
@@ -125,13 +284,15 @@ extern "C" int rgd_relbias_bwd(const rgd_relbias *bias, const void *dbias, int64
     if (!is_aligned(workspace, 16)) return RGD_E_STRIDE;
     relbias::BwdParams p{};
     p.borders = relbias::make_borders(*bias);
-    p.g = dbias; p.g_sh = stride_h; p.g_sq = stride_q; p.g_dtype = dtype;
+    p.g = dbias; p.g_sh = stride_h; p.g_sq = stride_q;
     p.dw = dweight; p.w_dtype = bias->dtype;
-    p.sums = reinterpret_cast<double *>(workspace);
+    p.parts = reinterpret_cast<float *>(workspace);
     p.H = (int)H; p.Tq = (int)Tq; p.Tk = (int)Tk; p.offset = (int)offset;
-    relbias::relbias_diagonals_kernel<<<dim3((unsigned)ceil_div64(Tq + Tk - 1, relbias::THREADS), (unsigned)H), relbias::THREADS, 0, st>>>(p);
-    count_launch();
-    relbias::relbias_buckets_kernel<<<dim3((unsigned)bias->num_buckets, (unsigned)H), relbias::THREADS, 0, st>>>(p);
-    count_launch();
-    return check_launch();
+    const relbias::BwdGrid grid = relbias::bwd_grid(H, Tq, Tk);
+    p.chunk = grid.chunk;
+    p.across = grid.across;
+    const int ve = 16 / dtype_size(dtype);
+    const bool vec = is_aligned(dbias, 16) && stride_h % ve == 0 && stride_q % ve == 0;
+    if (dtype == RGD_F32) return relbias::launch_bwd<float>(p, grid, vec, st);
+    return dtype == RGD_F16 ? relbias::launch_bwd<__half>(p, grid, vec, st) : relbias::launch_bwd<__nv_bfloat16>(p, grid, vec, st);
 }

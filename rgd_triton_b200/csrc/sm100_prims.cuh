@@ -150,6 +150,15 @@ __device__ __forceinline__ void bulk_load_1d(void *smem_dst, const void *gsrc, u
                  : "memory");
 }
 
+// Untiled bulk copy shared -> global, same rules; its bulk group is committed and waited for by the issuing thread.
+// The source must have been written through fence_proxy_async_smem() and a barrier.
+__device__ __forceinline__ void bulk_store_1d(void *gdst, const void *smem_src, uint32_t bytes) {
+    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(gdst), "r"(smem_u32(smem_src)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+// Until the sources of this thread's bulk stores have been read (their shared memory may then go away).
+__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+
 __device__ __forceinline__ void tma_prefetch_desc(const CUtensorMap *map) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
