@@ -4,12 +4,20 @@
 //   R(p): channels (2c, 2c + 1) -> (x0 cos - x1 sin, x1 cos + x0 sin) with the table's angles of position p.
 //
 // Every input is read once and every output written once.
+#include "attn_mma.cuh"
 #include "paged.cuh"
 
 namespace rgd {
 namespace paged {
 
 __device__ int g_append_status = 0;
+
+// How a CTA's threads lie over (token, head, channel group).
+struct AppendGeo {
+    int step, per_token, tokens;            // heads side by side, threads of a token, tokens side by side
+    int loop;                               // and one after another
+    FastDiv by_per_token;
+};
 
 struct AppendParams {
     PagedView view;
@@ -20,56 +28,213 @@ struct AppendParams {
     int64_t o_sb[3], o_sh[3], o_sn[3];
     const void *pos;                        // null: nothing is rotated
     int64_t pos_ss, pos_sn, P;
-    int pos_dtype, R;
+    int pos_dtype, R, pos_vec;              // pos_vec: the table's rows are 16-byte addressable
     int B, N, Hq, Hkv, d;
+    FastDiv by_n, by_vecs, by_groups;       // N, vecs, angle_groups
+    int vecs, angle_groups;                 // channel groups of a row; groups of 8 channels with a rotated one
+    AppendGeo geo[2];                       // of the caches, of the query
 };
 
-constexpr int APPEND_THREADS = 128;
+constexpr int APPEND_THREADS = 256;
+constexpr int APPEND_BATCH = 4;             // tokens that a thread reads before it uses the first
+constexpr int APPEND_LOOP = 8;              // most tokens of a thread
+constexpr int ANGLE_BYTES = 16 << 10;       // shared memory for the angles of a CTA's tokens
 
-// One CTA per token, a pair of neighbouring channels at a time.
-template <typename T>
-__global__ void __launch_bounds__(APPEND_THREADS) append_kernel(const __grid_constant__ AppendParams p) {
-    const int b = (int)(blockIdx.x / (unsigned)p.N), i = (int)(blockIdx.x - (unsigned)b * p.N);
-    const int count = p.counts ? p.counts[b] : p.N;
-    const int64_t position = (int64_t)p.lengths[b] + i;
-    bool live = i < count;
-    int page = 0, slot = 0;
-    if (live) {
-        bool ok = position >= 0 && position < capacity(p.view) && (!p.pos || position < p.P);
-        if (ok) {
-            int index;
-            split_position(p.view, (uint32_t)position, index, slot);
-            page = p.view.table[(int64_t)b * p.view.table_stride + index];
-            ok = page_ok(p.view, page);
+// Eight angles of a table row from element `at` on, `left` of them in the table, `past` in place of the others.
+__device__ __forceinline__ void load_angles(const AppendParams &p, int64_t at, int left, float past, float (&w)[8]) {
+    if (p.pos_vec && left >= 8) {
+        if (p.pos_dtype == RGD_F32) {
+            const float4 *f = reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(p.pos) + at);
+            const float4 a = f[0], b = f[1];
+            w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+            w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
+        } else if (p.pos_dtype == RGD_F16) {
+            const Vec<__half, 8> x = load_vec<__half, 8>(reinterpret_cast<const __half *>(p.pos) + at);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e] = __half2float(x.v[e]);
+        } else {
+            const Vec<__nv_bfloat16, 8> x = load_vec<__nv_bfloat16, 8>(reinterpret_cast<const __nv_bfloat16 *>(p.pos) + at);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e] = __bfloat162float(x.v[e]);
         }
-        if (!ok) {
-            live = false;
-            if (threadIdx.x == 0) g_append_status = 1;
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = e < left ? load_as_f32(p.pos, at + e, p.pos_dtype) : past;
+}
+
+// Where a token goes.
+struct alignas(16) Place {
+    int64_t out;                            // element offset of its head 0
+    int position;                           // -1: a key or value that is not written, a query that is copied
+};
+
+// Each CTA has one of the three tensors and a few tokens of it, each thread one group of VE channels (16 bytes, or a
+// pair where views are not addressable that way) of one head after another.  Where the tokens go and their angles are
+// looked up once for the CTA, two dependent reads (length; table entry and angles) during which the first tokens are on
+// their way; the loop is then read, turn, write.  [4, 4096, 16, 128] bf16 keys, values and queries (411 MB): 78 us, 81 %
+// of the copy rate, bound by instruction issue (two thirds of the slots busy) and the look-ups.  With every thread
+// looking up its own tokens it executed 222 instructions per 16 bytes instead of 130 and took 160-200 us.
+template <typename T, int VE>
+__global__ void __launch_bounds__(APPEND_THREADS, 5) append_kernel(const __grid_constant__ AppendParams p) {
+    using V = Vec<T, VE>;
+    extern __shared__ __align__(16) unsigned char raw[];
+    const int which = blockIdx.y, tid = threadIdx.x;
+    const AppendGeo &g = p.geo[which == 2];
+    const int heads = which == 2 ? p.Hq : p.Hkv, all = p.B * p.N, mine = g.loop * g.tokens;
+    const int first = blockIdx.x * mine;
+    if (first >= all || heads == 0) return;
+    Place *places = reinterpret_cast<Place *>(raw);             // [loop][tokens]
+    // [loop][tokens], sines and cosines, first and second halves of the groups of 8 channels (a warp then reads 16 bytes
+    // next to 16 bytes); channels past R have sine 0 and cosine 1
+    float *angles = reinterpret_cast<float *>(places + mine);
+    const int sub = (int)fdiv((uint32_t)tid, g.by_per_token), rest = tid - sub * g.per_token;
+    const int row0 = (int)fdiv((uint32_t)rest, p.by_vecs), c = (rest - row0 * p.vecs) * VE;
+    const bool works = sub < g.tokens;
+    const T *x = reinterpret_cast<const T *>(p.x[which]) + c;
+    T *out = reinterpret_cast<T *>(p.out[which]) + c;
+    const int64_t x_sb = p.x_sb[which], x_sh = p.x_sh[which], x_sn = p.x_sn[which], o_sh = p.o_sh[which];
+
+    // The thread's tokens are g.tokens apart, most often in one sequence: the first one's place in the input is worked
+    // out, the others' follow it unless a sequence ends between them.
+    const int64_t x_step = g.tokens * x_sn;
+    V v[APPEND_BATCH];
+    auto read = [&](int row, int t0) {
+        int token = first + t0 * g.tokens + sub, b = (int)fdiv((uint32_t)token, p.by_n), i = token - b * p.N;
+        const T *from = x + b * x_sb + row * x_sh + i * x_sn;
+#pragma unroll
+        for (int u = 0; u < APPEND_BATCH; ++u) {
+            if (t0 + u < g.loop && token < all) {
+                if constexpr (VE == 8) {
+                    v[u] = load_vec_stream<T, VE>(from);
+                } else {
+                    v[u].v[0] = from[0];
+                    v[u].v[1] = c + 1 < p.d ? from[1] : from_f32<T>(0.f);
+                }
+            }
+            token += g.tokens;
+            i += g.tokens;
+            from += x_step;
+            if (i >= p.N) {
+                b = (int)fdiv((uint32_t)token, p.by_n);
+                i = token - b * p.N;
+                from = x + b * x_sb + row * x_sh + i * x_sn;
+            }
+        }
+    };
+    if (works) read(row0, 0);
+
+    // position of token first + e, -1 when it is not a new one, -2 when it has none
+    auto position_of = [&](int e) -> int {
+        const int b = (int)fdiv((uint32_t)(first + e), p.by_n), i = first + e - b * p.N;
+        if (i >= (p.counts ? p.counts[b] : p.N)) return -1;
+        const int64_t position = (int64_t)p.lengths[b] + i;
+        return position >= 0 && position < capacity(p.view) && (!p.pos || position < p.P) ? (int)position : -2;
+    };
+    for (int e = tid; e < mine && first + e < all; e += APPEND_THREADS) {
+        const int b = (int)fdiv((uint32_t)(first + e), p.by_n), i = first + e - b * p.N;
+        Place at{which == 2 ? b * p.o_sb[2] + i * p.o_sn[2] : 0, position_of(e)};
+        if (at.position >= 0) {
+            int index, slot;
+            split_position(p.view, (uint32_t)at.position, index, slot);
+            const int page = p.view.table[b * p.view.table_stride + index];
+            if (!page_ok(p.view, page)) at.position = -2;
+            else if (which != 2) at.out = page * p.o_sb[which] + slot * p.o_sn[which];
+        }
+        if (at.position == -2) g_append_status = 1;
+        places[e] = at;
+    }
+    const bool turned = p.pos && which != 1;
+    if (turned) {
+        // one thread per token, sine or cosine, and group of 8 channels; it finds the position itself, so that the
+        // angles are read beside the table
+        const int groups = p.angle_groups;
+        for (int e = APPEND_THREADS - 1 - tid; e < mine * 2 * groups; e += APPEND_THREADS) {
+            const int t = (int)fdiv((uint32_t)e, p.by_groups) >> 1, r = e - t * 2 * groups, cosine = r >= groups, q = r - cosine * groups;
+            const int position = first + t < all ? position_of(t) : -1;
+            if (position < 0) continue;
+            float w[8];
+            load_angles(p, position * p.pos_sn + cosine * p.pos_ss + q * 8, p.R - q * 8, cosine ? 1.f : 0.f, w);
+            float *to = angles + (t * 2 + cosine) * 8 * groups + q * 4;
+            *reinterpret_cast<float4 *>(to) = make_float4(w[0], w[1], w[2], w[3]);
+            *reinterpret_cast<float4 *>(to + 4 * groups) = make_float4(w[4], w[5], w[6], w[7]);
         }
     }
-    const int pairs = (p.d + 1) / 2;
-    for (int t = threadIdx.x; t < (2 * p.Hkv + p.Hq) * pairs; t += APPEND_THREADS) {
-        const int row = t / pairs, c = (t - row * pairs) * 2;
-        const int which = row < p.Hkv ? 0 : row < 2 * p.Hkv ? 1 : 2, h = row - (which == 0 ? 0 : which * p.Hkv);
-        if (!live && which != 2) continue;
-        const T *x = reinterpret_cast<const T *>(p.x[which]) + (int64_t)b * p.x_sb[which] + (int64_t)h * p.x_sh[which] +
-                     (int64_t)i * p.x_sn[which] + c;
-        T *out = reinterpret_cast<T *>(p.out[which]) + (int64_t)h * p.o_sh[which] + c +
-                 (which == 2 ? (int64_t)b * p.o_sb[2] + (int64_t)i * p.o_sn[2]
-                             : (int64_t)page * p.o_sb[which] + (int64_t)slot * p.o_sn[which]);
-        const bool both = c + 1 < p.d;
-        T y0 = x[0], y1 = both ? x[1] : from_f32<T>(0.f);
-        if (live && which != 1 && c < p.R) {        // R is even: a rotated pair is whole
-            const int64_t at = position * p.pos_sn + c;
-            const float s0 = load_as_f32(p.pos, at, p.pos_dtype), s1 = load_as_f32(p.pos, at + 1, p.pos_dtype);
-            const float c0 = load_as_f32(p.pos, p.pos_ss + at, p.pos_dtype), c1 = load_as_f32(p.pos, p.pos_ss + at + 1, p.pos_dtype);
-            const float x0 = to_f32<T>(y0), x1 = to_f32<T>(y1);
-            y0 = from_f32<T>(x0 * c0 - x1 * s0);
-            y1 = from_f32<T>(x1 * c1 + x0 * s1);
+    __syncthreads();
+    if (!works) return;
+
+    const bool turns = turned && c < p.R;
+    const int quarter = 4 * p.angle_groups;                 // floats of one half of the groups
+    const float *sin0 = angles + sub * 4 * quarter + (c / 8) * 4 + (VE == 8 ? 0 : (c / 4) % 2 * quarter + c % 4);
+    for (int row = row0; row < heads; row += g.step) {
+        T *out_row = out + row * o_sh;
+        for (int t0 = 0; t0 < g.loop; t0 += APPEND_BATCH) {
+            if (row != row0 || t0 != 0) read(row, t0);
+#pragma unroll
+            for (int u = 0; u < APPEND_BATCH; ++u) {
+                const int t = (t0 + u) * g.tokens + sub;
+                if (t0 + u >= g.loop || first + t >= all) break;
+                const Place at = places[t];
+                if (at.position < 0 && which != 2) continue;
+                if (turns && at.position >= 0) {
+                    const float *sin = sin0 + (t0 + u) * g.tokens * 4 * quarter, *cos = sin + 2 * quarter;
+#pragma unroll
+                    for (int e = 0; e < VE; e += 4) {
+                        using W = Vec<float, VE == 8 ? 4 : 2>;
+                        const W sw = *reinterpret_cast<const W *>(sin + e / 4 * quarter), cw = *reinterpret_cast<const W *>(cos + e / 4 * quarter);
+#pragma unroll
+                        for (int k = 0; k < (VE == 8 ? 4 : 2); k += 2) {
+                            const float x0 = to_f32<T>(v[u].v[e + k]), x1 = to_f32<T>(v[u].v[e + k + 1]);
+                            *reinterpret_cast<uint32_t *>(&v[u].v[e + k]) =
+                                attn::Mma<T>::pack(x0 * cw.v[k] - x1 * sw.v[k], x1 * cw.v[k + 1] + x0 * sw.v[k + 1]);
+                        }
+                    }
+                }
+                T *to = out_row + at.out;
+                if constexpr (VE == 8) {
+                    store_vec<T, VE>(to, v[u]);
+                } else {
+                    to[0] = v[u].v[0];
+                    if (c + 1 < p.d) to[1] = v[u].v[1];
+                }
+            }
         }
-        out[0] = y0;
-        if (both) out[1] = y1;
     }
+}
+
+template <typename T, int VE>
+int launch_append(AppendParams &p, cudaStream_t st) {
+    p.vecs = (p.d + VE - 1) / VE;
+    p.by_vecs = make_fastdiv((uint32_t)p.vecs);
+    p.angle_groups = (p.R + 7) / 8;
+    p.by_groups = make_fastdiv(p.angle_groups > 0 ? (uint32_t)p.angle_groups : 1);
+    const int64_t all = (int64_t)p.B * p.N;
+    int64_t grid = 0;
+    size_t smem = 0;
+    for (int q = 0; q < 2; ++q) {
+        AppendGeo &g = p.geo[q];
+        const int heads = q ? p.Hq : p.Hkv;
+        if (heads == 0) continue;
+        g.step = APPEND_THREADS / p.vecs < heads ? APPEND_THREADS / p.vecs : heads;     // heads side by side
+        g.per_token = g.step * p.vecs;
+        g.tokens = APPEND_THREADS / g.per_token;
+        g.by_per_token = make_fastdiv((uint32_t)g.per_token);
+        // Tokens one after another: the look-ups of a CTA are worth about as much as two tokens (4 x 4096 tokens of 48
+        // heads: 180 us at one, 113 at two, 86 at four, 78 at eight, 80 at sixteen), but every SM should have four
+        // CTAs, and the angles have to fit.
+        const int64_t batches = ceil_div64(all, g.tokens), spread = batches * (p.Hq > 0 ? 3 : 2) / (4 * num_sms());
+        const size_t angle_bytes = (size_t)p.angle_groups * 16 * sizeof(float);
+        const int64_t fit = p.R > 0 ? (int64_t)(ANGLE_BYTES / (g.tokens * angle_bytes)) : APPEND_LOOP;
+        const int64_t loop = spread < fit ? spread : fit;
+        g.loop = (int)(loop < 1 ? 1 : loop > APPEND_LOOP ? APPEND_LOOP : loop);
+        const int64_t ctas = ceil_div64(batches, g.loop);
+        grid = ctas > grid ? ctas : grid;
+        const size_t bytes = (size_t)g.loop * g.tokens * (sizeof(Place) + angle_bytes);
+        smem = bytes > smem ? bytes : smem;
+    }
+    append_kernel<T, VE><<<dim3((unsigned)grid, p.Hq > 0 ? 3 : 2), APPEND_THREADS, smem, st>>>(p);
+    count_launch();
+    return check_launch();
 }
 
 int append_status_fetch() {
@@ -140,9 +305,14 @@ extern "C" int rgd_paged_append(const rgd_heads *key, const rgd_heads *value, co
     p.pos = R > 0 ? pos : nullptr;
     p.pos_ss = pos_stride_s; p.pos_sn = pos_stride_n; p.P = P; p.pos_dtype = pos_dtype; p.R = pos ? (int)R : 0;
     p.B = (int)B; p.N = (int)N; p.Hq = (int)Hq; p.Hkv = (int)Hkv; p.d = (int)d;
-    const unsigned grid = (unsigned)(B * N);
-    if (dtype == RGD_BF16) paged::append_kernel<__nv_bfloat16><<<grid, paged::APPEND_THREADS, 0, (cudaStream_t)stream>>>(p);
-    else paged::append_kernel<__half><<<grid, paged::APPEND_THREADS, 0, (cudaStream_t)stream>>>(p);
-    count_launch();
-    return check_launch();
+    p.by_n = make_fastdiv((uint32_t)N);
+    if (pos) {
+        const int ve = 16 / dtype_size(pos_dtype);
+        p.pos_vec = is_aligned(pos, 16) && pos_stride_s % ve == 0 && pos_stride_n % ve == 0;
+    }
+    const bool vec = d % 8 == 0 && (Hkv == 0 || (paged::cache_vec16(*cache) && paged::heads_vec16(*key) && paged::heads_vec16(*value))) &&
+                     (Hq == 0 || (paged::heads_vec16(*query) && paged::heads_vec16(*query_out)));
+    cudaStream_t st = (cudaStream_t)stream;
+    if (dtype == RGD_BF16) return vec ? paged::launch_append<__nv_bfloat16, 8>(p, st) : paged::launch_append<__nv_bfloat16, 2>(p, st);
+    return vec ? paged::launch_append<__half, 8>(p, st) : paged::launch_append<__half, 2>(p, st);
 }
