@@ -66,6 +66,7 @@ struct Smem {
     alignas(16) T v[STAGES][KEYS * LD];
     alignas(16) T p[2][ROWS * PLD];                     // weights, hi and lo
     float mx[2][WARPS][ROWS], l[WARPS][ROWS];
+    int64_t row[2][2][KEYS];                            // of the tiles to load next: element offsets of keys, of values; -1: none
     uint8_t live[STAGES][KEYS];                         // the key exists and its page is usable
     int64_t sums[WARPS];
     int64_t before;                                     // tiles before sequence `first`
@@ -103,7 +104,7 @@ __device__ __forceinline__ float *part_of(const AttnParams &p, int ctas, int D, 
 
 // Where a CTA stands in the tiles of all units.
 struct Cursor {
-    int b, unit, tile, tiles, len;
+    int b, hk, group, tile, tiles, len;
 };
 
 template <typename T, int D, bool VEC, bool BIAS>
@@ -156,21 +157,25 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D)) attn_kernel(const __g
         reinterpret_cast<Header *>(p.work)[cta].last = -1;
     }
 
-    Cursor at{}, to{};          // of the tile that is computed, of the tile that is loaded next
+    Cursor at{}, to{};          // of the tile that is computed, of the tile whose table entries are fetched next
     if (n > 0) {
         at.b = sm.first;
         at.len = live_length(p, at.b, false);
         at.tiles = tiles_of(at.len);
         const int64_t in = begin - sm.before * p.units;
-        at.unit = (int)(in / at.tiles);
-        at.tile = (int)(in - (int64_t)at.unit * at.tiles);
+        const int unit = (int)(in / at.tiles);
+        at.tile = (int)(in - (int64_t)unit * at.tiles);
+        at.hk = unit / p.groups;
+        at.group = unit - at.hk * p.groups;
         to = at;
     }
     auto advance = [&](Cursor &c) {
         if (++c.tile < c.tiles) return;
         c.tile = 0;
-        if (++c.unit < p.units) return;
-        c.unit = 0;
+        if (++c.group < p.groups) return;
+        c.group = 0;
+        if (++c.hk < p.Hkv) return;
+        c.hk = 0;
         for (++c.b; c.b < p.B; ++c.b) {
             c.len = live_length(p, c.b, false);
             c.tiles = tiles_of(c.len);
@@ -178,60 +183,72 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D)) attn_kernel(const __g
         }
     };
 
-    // Table entries of the rows that this thread copies of the tile at `to`: fetched one tile ahead of their use.
-    int entry[PASSES];
-    auto fetch = [&]() {
-        const int32_t *row = p.view.table + (int64_t)to.b * p.view.table_stride;
-#pragma unroll
-        for (int j = 0; j < PASSES; ++j) {
-            const int key = to.tile * KEYS + j * RPP + tid / CPR;
-            int index, slot;
-            split_position(p.view, (uint32_t)key, index, slot);
-            entry[j] = key < to.len ? row[index] : -1;
-        }
+    // Loading a tile takes three steps, a tile apart: a thread fetches the table entry of one key (the lower half of the
+    // CTA for keys, the upper one for values), works out where that row lies and leaves it in shared memory, and
+    // then all threads copy the rows, 16 bytes each.
+    const int my_key = tid % KEYS, my_half = tid / KEYS;
+    const int64_t my_sp = my_half ? p.v_sp : p.k_sp, my_ss = my_half ? p.v_ss : p.k_ss, my_sh = my_half ? p.v_sh : p.k_sh;
+    struct Fetched {
+        int entry, slot, hk;    // entry -1: nothing to read
     };
-    auto load = [&](int stage) {
-        const int hk = to.unit / p.groups;
-        const T *kh = reinterpret_cast<const T *>(p.k) + (int64_t)hk * p.k_sh, *vh = reinterpret_cast<const T *>(p.v) + (int64_t)hk * p.v_sh;
-        const int c = (tid % CPR) * 8;
-#pragma unroll
-        for (int j = 0; j < PASSES; ++j) {
-            const int r = j * RPP + tid / CPR, key = to.tile * KEYS + r;
-            const bool ok = key < to.len && page_ok(p.view, entry[j]);
-            int index, slot;
-            split_position(p.view, (uint32_t)key, index, slot);
-            const T *kr = kh, *vr = vh;
-            if (ok) {
-                kr += (int64_t)entry[j] * p.k_sp + (int64_t)slot * p.k_ss;
-                vr += (int64_t)entry[j] * p.v_sp + (int64_t)slot * p.v_ss;
-            } else if (key < to.len) {
+    auto fetch = [&]() {
+        Fetched f{-1, 0, to.hk};
+        const int key = to.tile * KEYS + my_key;
+        if (key < to.len) {
+            int index;
+            split_position(p.view, (uint32_t)key, index, f.slot);
+            f.entry = p.view.table[(int64_t)to.b * p.view.table_stride + index];
+            if (!page_ok(p.view, f.entry)) {
+                f.entry = -1;
                 g_attn_status = 1;
-            }
-            if (tid % CPR == 0) sm.live[stage][r] = ok;
-            T *kd = sm.k[stage] + r * LD + c, *vd = sm.v[stage] + r * LD + c;
-            if constexpr (VEC) {
-                const bool in = ok && c < p.d;
-                cp16(kd, in ? kr + c : kh, in);
-                cp16(vd, in ? vr + c : vh, in);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const bool in = ok && c + e < p.d;
-                    kd[e] = in ? kr[c + e] : from_f32<T>(0.f);
-                    vd[e] = in ? vr[c + e] : from_f32<T>(0.f);
-                }
             }
         }
         advance(to);
+        return f;
     };
-    if (n > 0) fetch();
+    auto find = [&](const Fetched &f, int i) {
+        sm.row[i & 1][my_half][my_key] = f.entry < 0 ? -1 : f.entry * my_sp + f.slot * my_ss + f.hk * my_sh;
+    };
+    auto load = [&](int i) {
+        const int stage = i % STAGES, c = (tid % CPR) * 8;
+        const T *kg = reinterpret_cast<const T *>(p.k) + c, *vg = reinterpret_cast<const T *>(p.v) + c;
 #pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) {
-        if (i < n) {
-            load(i);
-            if (i + 1 < n) fetch();
+        for (int j = 0; j < PASSES; ++j) {
+            const int r = j * RPP + tid / CPR;
+            const int64_t kr = sm.row[i & 1][0][r], vr = sm.row[i & 1][1][r];
+            T *kd = sm.k[stage] + r * LD + c, *vd = sm.v[stage] + r * LD + c;
+            if constexpr (VEC) {
+                const bool in = kr >= 0 && c < p.d;
+                cp16(kd, in ? kg + kr : p.k, in);
+                cp16(vd, in ? vg + vr : p.v, in);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const bool in = kr >= 0 && c + e < p.d;
+                    kd[e] = in ? kg[kr + e] : from_f32<T>(0.f);
+                    vd[e] = in ? vg[vr + e] : from_f32<T>(0.f);
+                }
+            }
         }
+        if (tid < KEYS) sm.live[stage][tid] = sm.row[i & 1][0][tid] >= 0;
+    };
+    static_assert(STAGES == 3, "the steps below are three tiles long");
+    Fetched next{};             // of tile i + STAGES once tile i is computed
+    {
+        Fetched f[STAGES];
+#pragma unroll
+        for (int i = 0; i < STAGES; ++i)
+            if (i < n) f[i] = fetch();
+        if (0 < n) find(f[0], 0);
+        if (1 < n) find(f[1], 1);
+        __syncthreads();
+        if (0 < n) load(0);
         asm volatile("cp.async.commit_group;" ::: "memory");
+        if (1 < n) load(1);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        __syncthreads();
+        if (2 < n) find(f[2], 2);
+        if (3 < n) next = fetch();
     }
 
     uint32_t aq[D / 16][4];             // the unit's queries as A fragments, rows past the group and channels past d as zeros
@@ -241,9 +258,8 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D)) attn_kernel(const __g
     const int mi = lane >> 3, mr = lane & 7;
 
     for (int i = 0; i < n; ++i) {
-        const int hk = at.unit / p.groups, row0 = (at.unit - hk * p.groups) * ROWS;
-        const int rows = min(ROWS, p.G - row0);
-        const int h0 = hk * p.G + row0;                 // query head of row 0
+        const int row0 = at.group * ROWS, rows = min(ROWS, p.G - row0);
+        const int h0 = at.hk * p.G + row0;              // query head of row 0
         const bool fresh = i == 0 || at.tile == 0;
         if (fresh) {
             whole = at.tile == 0;
@@ -271,11 +287,12 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D)) attn_kernel(const __g
         }
         asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
         __syncthreads();                // this tile has landed; the tile before it is done with
-        if (i + STAGES - 1 < n) {
-            load((i + STAGES - 1) % STAGES);
-            if (i + STAGES < n) fetch();
-        }
+        if (i + STAGES - 1 < n) load(i + STAGES - 1);
         asm volatile("cp.async.commit_group;" ::: "memory");
+        if (i + STAGES < n) {
+            find(next, i + STAGES);
+            if (i + STAGES + 1 < n) next = fetch();
+        }
         if constexpr (BIAS)
             if (fresh) {
                 for (int e = tid; e < p.borders.side * ROWS; e += THREADS) {
@@ -414,7 +431,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D)) attn_kernel(const __g
                 Header &head = reinterpret_cast<Header *>(p.work)[cta];
                 head.last = (int)(((t + 1) * busy - 1) / total);
                 head.b = at.b;
-                head.hk = hk;
+                head.hk = at.hk;
                 head.row0 = row0;
             }
         }
