@@ -45,36 +45,45 @@ __device__ __forceinline__ int live_length(const AttnParams &p, int b, bool repo
 
 // ---------------------------------------------------------------------------------------------------------------
 // Work.  A unit is a sequence, a cache head and up to 16 of the query heads that share it (one m16n8k16 row tile);
-// its keys come in tiles of 64.  The tiles of all units, one after the other, are dealt out to the CTAs in equal
-// runs, whatever the lengths are: each CTA finds its run from the lengths, which are on the device.  A unit that one
-// CTA has whole is finished there; of a unit that several have, each leaves its part (row maximum, row sum,
+// its keys come in tiles.  The tiles of all units, one after the other, are dealt out to the warps of the grid in runs
+// of equal cost, whatever the lengths are; a CTA finds its warps' runs from the lengths, which are on the device.  A unit
+// that one warp has whole is finished there; of a unit that several have, each leaves its part (row maximum, row sum,
 // unnormalised output) in the workspace, and join_kernel adds the parts in order.
 //
-// A CTA streams its run through a ring of cp.async stages that goes on across units.  Of a tile, each of the four
-// warps takes the scores of 16 keys; the row maxima and the weights are exchanged through shared memory, and each
-// warp then adds the products with all 64 values for a quarter of the channels, so no partial outputs have to be
-// added up between the warps.  Weights are split into two numbers of the cache's type (hi + lo): rounded to one, they
-// would cost as much accuracy as the output's own rounding, and the matrix pipe idles anyway.
+// A warp does everything for its tiles: it streams the keys and values through a ring of cp.async stages of its own,
+// which goes on across units, keeps the running maximum, sum and output in registers, and waits for no other warp.
+// Two forms in which the four warps of a CTA shared a unit were slower: with the maxima and weights of a tile exchanged
+// and the channels split, three barriers a tile held the loop (120 us for one sequence of 131 thousand keys, 93 us like
+// this); with 16 keys of a tile each, added up at the unit's end, short sequences paid for that (103 us for 64 of 16
+// to 8192 keys).
+//
+// Weights are split into two numbers of the cache's type (hi + lo): rounded to one, they would cost as much accuracy
+// as the output's own rounding, and the matrix pipe idles anyway.
 // ---------------------------------------------------------------------------------------------------------------
-constexpr int WARPS = 4, THREADS = WARPS * 32, KEYS = 64, ROWS = 16, STAGES = 3, PLD = KEYS + attn::PAD;
-constexpr int MIN_TILES = 1;
+constexpr int WARPS = 4, THREADS = WARPS * 32, ROWS = 16, STAGES = 3, CTAS_PER_SM = 2;
+constexpr int UNIT_COST = 2;            // of a unit's queries and output, in tiles
+constexpr int MIN_COST = 6;             // least run of a warp
+
+__host__ __device__ constexpr int tile_keys(int D) { return D > 64 ? 16 : 32; }      // 8 KB of keys and values
 
 template <typename T, int D>
 struct Smem {
-    static constexpr int LD = D + attn::PAD;            // rows 16 bytes apart from bank to bank: conflict-free ldmatrix
-    alignas(16) T k[STAGES][KEYS * LD];
-    alignas(16) T v[STAGES][KEYS * LD];
-    alignas(16) T p[2][ROWS * PLD];                     // weights, hi and lo
-    float mx[2][WARPS][ROWS], l[WARPS][ROWS];
-    int64_t row[2][2][KEYS];                            // of the tiles to load next: element offsets of keys, of values; -1: none
-    uint8_t live[STAGES][KEYS];                         // the key exists and its page is usable
+    static constexpr int KEYS = tile_keys(D);
+    // rows of D channels; the 16-byte chunks of row r change places by r mod 8, so that the rows of an ldmatrix lie in
+    // different banks
+    struct alignas(16) Stage {
+        T k[KEYS * D], v[KEYS * D];
+    };
+    Stage ring[WARPS][STAGES];
+    int64_t row[WARPS][2][2 * KEYS];                    // of the tiles to load next: element offsets of keys, of values; -1: none
     int64_t sums[WARPS];
-    int64_t before;                                     // tiles before sequence `first`
-    int first;
-    float bias[1];                                      // [side][ROWS], with a position bias
+    int counts[WARPS];
+    struct Boundary {                                   // where a warp's run begins
+        int64_t tiles;                                  // of all units before it
+        int b, unit, tile;
+    } at[WARPS + 1];
+    int borders[relbias::MAX_SIDE];                     // with a position bias
 };
-
-__host__ __device__ constexpr int ctas_per_sm(int D) { return D > 64 ? 2 : 3; }
 
 __device__ __forceinline__ void cp16(void *dst, const void *src, bool valid) {
     // not valid: nothing is read, 16 zero bytes are written
@@ -86,87 +95,113 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ int tiles_of(int len) { return (len + KEYS - 1) / KEYS; }
 
-// Workspace: per CTA of the grid a header and two parts, [0] of a unit that began in another CTA's run, [1] of one
+// Workspace: per warp of the grid a header and two parts, [0] of a unit that began in another warp's run, [1] of one
 // that ends in another's.
 struct Header {
-    int last;                   // the unit of part [1] ends in this CTA; -1: there is none
+    int last;                   // the unit of part [1] ends in this warp; -1: there is none
     int b, hk, row0;
 };
 __host__ __device__ __forceinline__ int64_t part_floats(int D) { return ROWS * (D + 2); }
 __host__ __device__ __forceinline__ int64_t workspace_bytes(int ctas, int D) {
-    return (int64_t)ctas * ((int64_t)sizeof(Header) + 2 * part_floats(D) * (int64_t)sizeof(float));
+    return (int64_t)ctas * WARPS * ((int64_t)sizeof(Header) + 2 * part_floats(D) * (int64_t)sizeof(float));
 }
-__device__ __forceinline__ float *part_of(const AttnParams &p, int ctas, int D, int cta, int which) {
-    return reinterpret_cast<float *>(p.work + (int64_t)ctas * sizeof(Header)) + (cta * 2 + which) * part_floats(D);
+__device__ __forceinline__ float *part_of(const AttnParams &p, int warps, int D, int warp, int which) {
+    return reinterpret_cast<float *>(p.work + (int64_t)warps * sizeof(Header)) + (warp * 2 + which) * part_floats(D);
 }
 
-// Where a CTA stands in the tiles of all units.
+// Where a warp stands in the tiles of all units.
 struct Cursor {
     int b, hk, group, tile, tiles, len;
 };
 
 template <typename T, int D, bool VEC, bool BIAS>
-__global__ void __launch_bounds__(THREADS, ctas_per_sm(D)) attn_kernel(const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attn_kernel(const __grid_constant__ AttnParams p) {
     using S = Smem<T, D>;
-    constexpr int LD = S::LD, CPR = D / 8, RPP = THREADS / CPR, PASSES = KEYS / RPP, NT = D / 4 / 8;
+    constexpr int KEYS = S::KEYS, CPR = D / 8, RPP = 32 / CPR, PASSES = KEYS / RPP;      // 16-byte chunks of a row, rows a warp copies at once
+    constexpr int NT = D / 8, KT = KEYS / 8;                // column tiles of the output, of the scores
     extern __shared__ __align__(16) unsigned char raw[];
     S &sm = *reinterpret_cast<S *>(raw);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gq = lane >> 2, tq = lane & 3;
-    const int ctas = gridDim.x, cta = blockIdx.x;
+    const int warps = gridDim.x * WARPS, me = blockIdx.x * WARPS + warp;
     sm100::grid_trigger();
+    auto tiles_of = [](int len) { return (len + KEYS - 1) / KEYS; };
+    auto cost_of = [&](int tiles) { return tiles > 0 ? tiles + UNIT_COST : 0; };
 
-    // tiles per head before each sequence: every thread sums a run of sequences, then the runs are added up
+    // cost of a head's units before each sequence: every thread sums a run of sequences, then the runs are added up
     const int chunk = (p.B + THREADS - 1) / THREADS, b0 = min(tid * chunk, p.B), b1 = min(b0 + chunk, p.B);
-    int64_t mine = 0;
-    for (int b = b0; b < b1; ++b) mine += tiles_of(live_length(p, b, cta == 0));
-    int64_t upto = mine;
+    int64_t mine = 0, upto;
+    int filled = 0, filled_upto;                            // sequences with a token
+    for (int b = b0; b < b1; ++b) {
+        const int tiles = tiles_of(live_length(p, b, blockIdx.x == 0));
+        mine += cost_of(tiles);
+        filled += tiles > 0;
+    }
+    upto = mine;
+    filled_upto = filled;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += x;
+        const int y = __shfl_up_sync(0xffffffffu, filled_upto, o);
+        if (lane >= o) {
+            upto += x;
+            filled_upto += y;
+        }
     }
-    if (lane == 31) sm.sums[warp] = upto;
+    if (lane == 31) {
+        sm.sums[warp] = upto;
+        sm.counts[warp] = filled_upto;
+    }
+    if (BIAS)
+        for (int k = tid; k < p.borders.side - 1; k += THREADS) sm.borders[k] = p.borders.at[k];
     __syncthreads();
     int64_t all = 0;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) {
-        if (w < warp) upto += sm.sums[w];
+        if (w < warp) {
+            upto += sm.sums[w];
+            filled_upto += sm.counts[w];
+        }
         all += sm.sums[w];
     }
     const int64_t total = all * p.units;
-    const int64_t busy = min((int64_t)ctas, (total + MIN_TILES - 1) / MIN_TILES);      // CTAs with a run
-    const int64_t begin = cta < busy ? cta * total / busy : 0, end = cta < busy ? (cta + 1) * total / busy : 0;
-    const int n = (int)(end - begin);
-    if (n > 0) {
+    const int64_t busy = min((int64_t)warps, (total + MIN_COST - 1) / MIN_COST);       // warps with a run
+    // the boundaries of this CTA's runs: the thread whose sequences a boundary lies in finds it.  A unit's cost comes
+    // before its tiles.
+#pragma unroll
+    for (int w = 0; w <= WARPS; ++w) {
+        const int64_t first = min((int64_t)blockIdx.x * WARPS + w, busy);
+        const int64_t pos = busy > 0 ? first * total / busy : 0;
         int64_t before = upto - mine;
-        if (begin >= before * p.units && begin < upto * p.units)
+        int64_t filled_before = filled_upto - filled;
+        if (pos >= before * p.units && pos < upto * p.units) {
             for (int b = b0; b < b1; ++b) {
-                const int64_t next = before + tiles_of(live_length(p, b, false));
-                if (begin < next * p.units) {
-                    sm.first = b;
-                    sm.before = before;
+                const int tiles = tiles_of(live_length(p, b, false)), cost = cost_of(tiles);
+                if (pos < (before + cost) * p.units) {
+                    const int64_t in = pos - before * p.units;
+                    const int unit = (int)(in / cost), tile = max((int)(in - (int64_t)unit * cost) - UNIT_COST, 0);
+                    sm.at[w] = {(before - filled_before * UNIT_COST) * p.units + (int64_t)unit * tiles + tile, b, unit, tile};
                     break;
                 }
-                before = next;
+                before += cost;
+                filled_before += tiles > 0;
             }
+        } else if (tid == THREADS - 1 && pos >= total) {
+            sm.at[w] = {(all - (int64_t)filled_upto * UNIT_COST) * p.units, p.B, 0, 0};
+        }
     }
     __syncthreads();
-    if (tid == 0) {
-        reinterpret_cast<Header *>(p.work)[cta].last = -1;
-    }
+    const int n = (int)(sm.at[warp + 1].tiles - sm.at[warp].tiles);
+    if (lane == 0) reinterpret_cast<Header *>(p.work)[me].last = -1;
 
     Cursor at{}, to{};          // of the tile that is computed, of the tile whose table entries are fetched next
     if (n > 0) {
-        at.b = sm.first;
+        at.b = sm.at[warp].b;
         at.len = live_length(p, at.b, false);
         at.tiles = tiles_of(at.len);
-        const int64_t in = begin - sm.before * p.units;
-        const int unit = (int)(in / at.tiles);
-        at.tile = (int)(in - (int64_t)unit * at.tiles);
-        at.hk = unit / p.groups;
-        at.group = unit - at.hk * p.groups;
+        at.tile = sm.at[warp].tile;
+        at.hk = sm.at[warp].unit / p.groups;
+        at.group = sm.at[warp].unit - at.hk * p.groups;
         to = at;
     }
     auto advance = [&](Cursor &c) {
@@ -183,40 +218,42 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D)) attn_kernel(const __g
         }
     };
 
-    // Loading a tile takes three steps, a tile apart: a thread fetches the table entry of one key (the lower half of the
-    // CTA for keys, the upper one for values), works out where that row lies and leaves it in shared memory, and
-    // then all threads copy the rows, 16 bytes each.
-    const int my_key = tid % KEYS, my_half = tid / KEYS;
-    const int64_t my_sp = my_half ? p.v_sp : p.k_sp, my_ss = my_half ? p.v_ss : p.k_ss, my_sh = my_half ? p.v_sh : p.k_sh;
-    struct Fetched {
-        int entry, slot, hk;    // entry -1: nothing to read
-    };
+    // Loading a tile takes three steps, a tile apart: a lane fetches the table entry of one key, works out where its row
+    // (of keys and of values; of one of them where there are 16 keys) lies and leaves that in shared memory, and then
+    // all lanes copy the rows, 16 bytes each.
+    const int my_key = lane % KEYS;
+    int entry = -1, slot = 0, entry_hk = 0;     // fetched; entry -1: nothing to read
+    uint32_t live[STAGES + 1] = {};             // which of the keys of tile i, i + 1, ... there are
     auto fetch = [&]() {
-        Fetched f{-1, 0, to.hk};
         const int key = to.tile * KEYS + my_key;
+        entry = -1;
+        entry_hk = to.hk;
         if (key < to.len) {
             int index;
-            split_position(p.view, (uint32_t)key, index, f.slot);
-            f.entry = p.view.table[(int64_t)to.b * p.view.table_stride + index];
-            if (!page_ok(p.view, f.entry)) {
-                f.entry = -1;
+            split_position(p.view, (uint32_t)key, index, slot);
+            entry = p.view.table[(int64_t)to.b * p.view.table_stride + index];
+            if (!page_ok(p.view, entry)) {
+                entry = -1;
                 g_attn_status = 1;
             }
         }
         advance(to);
-        return f;
     };
-    auto find = [&](const Fetched &f, int i) {
-        sm.row[i & 1][my_half][my_key] = f.entry < 0 ? -1 : f.entry * my_sp + f.slot * my_ss + f.hk * my_sh;
+    auto find = [&](int i) {
+        if (KEYS == 32 || lane < KEYS) sm.row[warp][i & 1][lane] = entry < 0 ? -1 : entry * p.k_sp + slot * p.k_ss + entry_hk * p.k_sh;
+        if (KEYS == 32 || lane >= KEYS)
+            sm.row[warp][i & 1][KEYS + my_key] = entry < 0 ? -1 : entry * p.v_sp + slot * p.v_ss + entry_hk * p.v_sh;
+        return __ballot_sync(0xffffffffu, entry >= 0);
     };
     auto load = [&](int i) {
-        const int stage = i % STAGES, c = (tid % CPR) * 8;
+        typename S::Stage &st = sm.ring[warp][i % STAGES];
+        const int part = lane % CPR, c = part * 8;
         const T *kg = reinterpret_cast<const T *>(p.k) + c, *vg = reinterpret_cast<const T *>(p.v) + c;
 #pragma unroll
         for (int j = 0; j < PASSES; ++j) {
-            const int r = j * RPP + tid / CPR;
-            const int64_t kr = sm.row[i & 1][0][r], vr = sm.row[i & 1][1][r];
-            T *kd = sm.k[stage] + r * LD + c, *vd = sm.v[stage] + r * LD + c;
+            const int r = j * RPP + lane / CPR, to_c = r * D + (part ^ (r & 7)) * 8;
+            const int64_t kr = sm.row[warp][i & 1][r], vr = sm.row[warp][i & 1][KEYS + r];
+            T *kd = st.k + to_c, *vd = st.v + to_c;
             if constexpr (VEC) {
                 const bool in = kr >= 0 && c < p.d;
                 cp16(kd, in ? kg + kr : p.k, in);
@@ -230,38 +267,31 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D)) attn_kernel(const __g
                 }
             }
         }
-        if (tid < KEYS) sm.live[stage][tid] = sm.row[i & 1][0][tid] >= 0;
     };
     static_assert(STAGES == 3, "the steps below are three tiles long");
-    Fetched next{};             // of tile i + STAGES once tile i is computed
-    {
-        Fetched f[STAGES];
 #pragma unroll
-        for (int i = 0; i < STAGES; ++i)
-            if (i < n) f[i] = fetch();
-        if (0 < n) find(f[0], 0);
-        if (1 < n) find(f[1], 1);
-        __syncthreads();
-        if (0 < n) load(0);
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        if (1 < n) load(1);
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        __syncthreads();
-        if (2 < n) find(f[2], 2);
-        if (3 < n) next = fetch();
+    for (int i = 0; i < STAGES; ++i) {
+        if (i < n) {
+            fetch();
+            __syncwarp();
+            live[i] = find(i);
+            __syncwarp();
+            if (i < STAGES - 1) load(i);
+        }
+        if (i < STAGES - 1) asm volatile("cp.async.commit_group;" ::: "memory");
     }
+    if (STAGES < n) fetch();
 
     uint32_t aq[D / 16][4];             // the unit's queries as A fragments, rows past the group and channels past d as zeros
-    float o[NT][4];                     // rows gq and gq + 8, this warp's quarter of the channels
-    float m_ref[2], l_sum[2];           // the same in all warps; of this warp's keys
+    float o[NT][4];                     // rows gq and gq + 8
+    float m_ref[2], l_sum[2];
     bool whole = false;                 // the unit's first tile was in this run
     const int mi = lane >> 3, mr = lane & 7;
 
     for (int i = 0; i < n; ++i) {
         const int row0 = at.group * ROWS, rows = min(ROWS, p.G - row0);
         const int h0 = at.hk * p.G + row0;              // query head of row 0
-        const bool fresh = i == 0 || at.tile == 0;
-        if (fresh) {
+        if (i == 0 || at.tile == 0) {
             whole = at.tile == 0;
             const T *qg = reinterpret_cast<const T *>(p.q) + (int64_t)at.b * p.q_sb + (int64_t)h0 * p.q_sh;
 #pragma unroll
@@ -286,51 +316,45 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D)) attn_kernel(const __g
             l_sum[0] = l_sum[1] = 0.f;
         }
         asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
-        __syncthreads();                // this tile has landed; the tile before it is done with
+        __syncwarp();                   // this tile has landed; all lanes are done with the tile before it
         if (i + STAGES - 1 < n) load(i + STAGES - 1);
         asm volatile("cp.async.commit_group;" ::: "memory");
         if (i + STAGES < n) {
-            find(next, i + STAGES);
-            if (i + STAGES + 1 < n) next = fetch();
+            live[STAGES] = find(i + STAGES);
+            if (i + STAGES + 1 < n) fetch();
         }
-        if constexpr (BIAS)
-            if (fresh) {
-                for (int e = tid; e < p.borders.side * ROWS; e += THREADS) {
-                    const int r = e % ROWS;
-                    sm.bias[e] = r < rows ? attn::bias_log2<float>(load_as_f32(p.w, (e / ROWS) * p.w_sk + (h0 + r) * p.w_sh, p.w_dtype)) : 0.f;
-                }
-                __syncthreads();
-            }
-        const int stage = i % STAGES, par = i & 1;
-        const T *ks = sm.k[stage] + warp * 16 * LD, *vs = sm.v[stage] + warp * (D / 4);
+        const typename S::Stage &st = sm.ring[warp][i % STAGES];
 
-        float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+        float s[KT][4];
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-            uint32_t bf[4];
-            attn::ldmatrix_x4(bf, ks + (mr + (mi >> 1) * 8) * LD + kk * 16 + (mi & 1) * 8);
-            attn::Mma<T>::mma(s[0], aq[kk], bf[0], bf[1]);
-            attn::Mma<T>::mma(s[1], aq[kk], bf[2], bf[3]);
-        }
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[t][e] = 0.f;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk)
+#pragma unroll
+            for (int t = 0; t < KT; t += 2) {
+                uint32_t bf[4];
+                attn::ldmatrix_x4(bf, st.k + (t * 8 + mr + (mi >> 1) * 8) * D + ((kk * 2 + (mi & 1)) ^ mr) * 8);
+                attn::Mma<T>::mma(s[t], aq[kk], bf[0], bf[1]);
+                attn::Mma<T>::mma(s[t + 1], aq[kk], bf[2], bf[3]);
+            }
         int bucket = 0;
-        if constexpr (BIAS) {
-            const int key = at.tile * KEYS + warp * 16 + (lane & 15);
-            bucket = relbias::bucket_of_distance(p.borders.at, p.borders.side, max(at.len - 1 - key, 0));
-        }
+        if constexpr (BIAS) bucket = relbias::bucket_of_distance(sm.borders, p.borders.side, max(at.len - 1 - (at.tile * KEYS + my_key), 0));
         float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < KT; ++t)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int key = t * 8 + tq * 2 + e;
-                const bool live = sm.live[stage][warp * 16 + key];
-                int bk = 0;
-                if constexpr (BIAS) bk = __shfl_sync(0xffffffffu, bucket, key) * ROWS;
+                int64_t w_at = 0;
+                if constexpr (BIAS) w_at = __shfl_sync(0xffffffffu, bucket, key) * p.w_sk + (h0 + gq) * p.w_sh;
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
                     float x = s[t][r * 2 + e] * p.scale_log2;
-                    if constexpr (BIAS) x += sm.bias[bk + gq + r * 8];
-                    x = live ? x : -INFINITY;
+                    if constexpr (BIAS)
+                        if (gq + r * 8 < rows) x += attn::bias_log2<float>(load_as_f32(p.w, w_at + r * 8 * p.w_sh, p.w_dtype));
+                    if (!(live[0] >> key & 1)) x = -INFINITY;
                     s[t][r * 2 + e] = x;
                     mx[r] = fmaxf(mx[r], x);
                 }
@@ -339,71 +363,64 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D)) attn_kernel(const __g
         for (int r = 0; r < 2; ++r) {
             mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
             mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
-            if (tq == 0) sm.mx[par][warp][gq + r * 8] = mx[r];
         }
-        __syncthreads();
+        // the reference follows the maximum: a new one gets rare along the keys
+        const bool more[2] = {mx[0] > m_ref[0], mx[1] > m_ref[1]};
+        if (__any_sync(0xffffffffu, more[0] || more[1])) {
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const int row = gq + r * 8;
-            float m_new = m_ref[r];
+            for (int r = 0; r < 2; ++r) {
+                const float alpha = !more[r] ? 1.f : m_ref[r] == -INFINITY ? 0.f : ex2(m_ref[r] - mx[r]);
+                if (more[r]) m_ref[r] = mx[r];
+                l_sum[r] *= alpha;
 #pragma unroll
-            for (int w = 0; w < WARPS; ++w) m_new = fmaxf(m_new, sm.mx[par][w][row]);
-            const float mu = m_new == -INFINITY ? 0.f : m_new, alpha = ex2(m_ref[r] - mu);
-            m_ref[r] = m_new;
-            l_sum[r] *= alpha;
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                o[j][2 * r] *= alpha;
-                o[j][2 * r + 1] *= alpha;
-            }
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const float p0 = ex2(s[t][2 * r] - mu), p1 = ex2(s[t][2 * r + 1] - mu);
-                l_sum[r] += p0 + p1;
-                const float r0 = round_to<T>(p0), r1 = round_to<T>(p1);
-                const int e = row * PLD + warp * 16 + t * 8 + tq * 2;
-                *reinterpret_cast<uint32_t *>(&sm.p[0][e]) = attn::Mma<T>::pack(r0, r1);
-                *reinterpret_cast<uint32_t *>(&sm.p[1][e]) = attn::Mma<T>::pack(p0 - r0, p1 - r1);
+                for (int j = 0; j < NT; ++j) {
+                    o[j][2 * r] *= alpha;
+                    o[j][2 * r + 1] *= alpha;
+                }
             }
         }
-        __syncthreads();
 #pragma unroll
-        for (int kk = 0; kk < KEYS / 16; ++kk) {
+        for (int kk = 0; kk < KT / 2; ++kk) {
             uint32_t hi[4], lo[4];
-            attn::ldmatrix_x4(hi, sm.p[0] + (lane & 15) * PLD + kk * 16 + (lane >> 4) * 8);
-            attn::ldmatrix_x4(lo, sm.p[1] + (lane & 15) * PLD + kk * 16 + (lane >> 4) * 8);
 #pragma unroll
-            for (int j = 0; j < NT / 2; ++j) {
+            for (int r = 0; r < 2; ++r) {
+                const float mu = m_ref[r] == -INFINITY ? 0.f : m_ref[r];
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const float p0 = ex2(s[2 * kk + t][2 * r] - mu), p1 = ex2(s[2 * kk + t][2 * r + 1] - mu);
+                    l_sum[r] += p0 + p1;
+                    const float r0 = round_to<T>(p0), r1 = round_to<T>(p1);
+                    hi[t * 2 + r] = attn::Mma<T>::pack(r0, r1);
+                    lo[t * 2 + r] = attn::Mma<T>::pack(p0 - r0, p1 - r1);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < NT; j += 2) {
                 uint32_t bf[4];
-                attn::ldmatrix_x4_trans(bf, vs + (kk * 16 + mr + (mi & 1) * 8) * LD + j * 16 + (mi >> 1) * 8);
-                attn::Mma<T>::mma(o[2 * j], hi, bf[0], bf[1]);
-                attn::Mma<T>::mma(o[2 * j + 1], hi, bf[2], bf[3]);
-                attn::Mma<T>::mma(o[2 * j], lo, bf[0], bf[1]);
-                attn::Mma<T>::mma(o[2 * j + 1], lo, bf[2], bf[3]);
+                attn::ldmatrix_x4_trans(bf, st.v + (kk * 16 + mr + (mi & 1) * 8) * D + ((j + (mi >> 1)) ^ mr) * 8);
+                attn::Mma<T>::mma(o[j], hi, bf[0], bf[1]);
+                attn::Mma<T>::mma(o[j + 1], hi, bf[2], bf[3]);
+                attn::Mma<T>::mma(o[j], lo, bf[0], bf[1]);
+                attn::Mma<T>::mma(o[j + 1], lo, bf[2], bf[3]);
             }
         }
+#pragma unroll
+        for (int j = 0; j < STAGES; ++j) live[j] = live[j + 1];
 
         const bool done = at.tile == at.tiles - 1;
         if (done || i == n - 1) {
-            // row sums over the warps; the next tile's barriers keep sm.l until everyone has read it
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
                 l_sum[r] += __shfl_xor_sync(0xffffffffu, l_sum[r], 1);
                 l_sum[r] += __shfl_xor_sync(0xffffffffu, l_sum[r], 2);
-                if (tq == 0) sm.l[warp][gq + r * 8] = l_sum[r];
-            }
-            __syncthreads();
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
                 const int row = gq + r * 8;
                 if (row >= rows) continue;
-                const float L = (sm.l[0][row] + sm.l[1][row]) + (sm.l[2][row] + sm.l[3][row]);
                 if (done && whole) {
-                    const float inv = L == 0.f ? 0.f : 1.f / L;
+                    const float inv = l_sum[r] == 0.f ? 0.f : 1.f / l_sum[r];
                     T *out = reinterpret_cast<T *>(p.o) + (int64_t)at.b * p.o_sb + (int64_t)(h0 + row) * p.o_sh;
 #pragma unroll
                     for (int j = 0; j < NT; ++j) {
-                        const int c = warp * (D / 4) + j * 8 + tq * 2;
+                        const int c = j * 8 + tq * 2;
                         if constexpr (VEC) {
                             if (c < p.d) *reinterpret_cast<uint32_t *>(out + c) = attn::Mma<T>::pack(o[j][2 * r] * inv, o[j][2 * r + 1] * inv);
                         } else {
@@ -411,24 +428,24 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D)) attn_kernel(const __g
                             if (c + 1 < p.d) out[c + 1] = from_f32<T>(o[j][2 * r + 1] * inv);
                         }
                     }
-                    if (p.lse && warp == 0 && tq == 0)
-                        p.lse[(int64_t)at.b * p.Hq + h0 + row] = L == 0.f ? -INFINITY : (m_ref[r] + log2f(L)) * LN2;
+                    if (p.lse && tq == 0)
+                        p.lse[(int64_t)at.b * p.Hq + h0 + row] = l_sum[r] == 0.f ? -INFINITY : (m_ref[r] + log2f(l_sum[r])) * LN2;
                 } else {
-                    float *part = part_of(p, ctas, D, cta, whole ? 1 : 0);
-                    if (warp == 0 && tq == 0) {
+                    float *part = part_of(p, warps, D, me, whole ? 1 : 0);
+                    if (tq == 0) {
                         part[row] = m_ref[r];
-                        part[ROWS + row] = L;
+                        part[ROWS + row] = l_sum[r];
                     }
 #pragma unroll
                     for (int j = 0; j < NT; ++j)
-                        *reinterpret_cast<float2 *>(part + 2 * ROWS + row * D + warp * (D / 4) + j * 8 + tq * 2) =
-                            make_float2(o[j][2 * r], o[j][2 * r + 1]);
+                        *reinterpret_cast<float2 *>(part + 2 * ROWS + row * D + j * 8 + tq * 2) = make_float2(o[j][2 * r], o[j][2 * r + 1]);
                 }
             }
-            if (!done && whole && tid == 0) {
-                // the run that has the unit's last tile: cta * total / busy <= t < (cta + 1) * total / busy
-                const int64_t t = end - 1 + (at.tiles - 1 - at.tile);
-                Header &head = reinterpret_cast<Header *>(p.work)[cta];
+            if (!done && whole && lane == 0) {
+                // The warp that has the unit's last tile: this run ends at cost position (me + 1) * total / busy, the
+                // unit as many tiles later as are left, and warp x's run is [x * total / busy, (x + 1) * total / busy).
+                const int64_t t = (me + 1) * total / busy - 1 + (at.tiles - 1 - at.tile);
+                Header &head = reinterpret_cast<Header *>(p.work)[me];
                 head.last = (int)(((t + 1) * busy - 1) / total);
                 head.b = at.b;
                 head.hk = at.hk;
@@ -440,7 +457,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D)) attn_kernel(const __g
     asm volatile("cp.async.wait_group 0;" ::: "memory");
 
     // sequences without a token
-    for (int b = cta; b < p.B; b += ctas)
+    for (int b = blockIdx.x; b < p.B; b += gridDim.x)
         if (live_length(p, b, false) == 0) {
             T *out = reinterpret_cast<T *>(p.o) + (int64_t)b * p.o_sb;
             for (int e = tid; e < p.Hq * p.d; e += THREADS) {
@@ -452,80 +469,87 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D)) attn_kernel(const __g
         }
 }
 
-// Adds the parts of the unit that begins in CTA blockIdx.x's run and ends in another's; one CTA per row.
+constexpr int JOIN_THREADS = 256, JOIN_WARPS = JOIN_THREADS / 32;
+
+// Adds the parts of the units that begin in the runs of the attention's CTA blockIdx.x and end in other warps'; one CTA
+// per row.
 template <typename T, int D>
-__global__ void __launch_bounds__(THREADS) join_kernel(const __grid_constant__ AttnParams p) {
-    constexpr int QUADS = D / 4, GROUPS = THREADS / QUADS;
-    __shared__ float red[WARPS], l_s[GROUPS];
+__global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const __grid_constant__ AttnParams p) {
+    constexpr int QUADS = D / 4, GROUPS = JOIN_THREADS / QUADS;
+    __shared__ float red[JOIN_WARPS], l_s[GROUPS];
     __shared__ float4 acc_s[GROUPS][QUADS];
-    const int tid = threadIdx.x, quad = tid % QUADS, grp = tid / QUADS, cta = blockIdx.x, row = blockIdx.y, ctas = gridDim.x;
+    const int tid = threadIdx.x, quad = tid % QUADS, grp = tid / QUADS, row = blockIdx.y, warps = gridDim.x * WARPS;
     sm100::grid_wait();
-    const Header head = reinterpret_cast<const Header *>(p.work)[cta];
-    if (head.last < 0 || row >= min(ROWS, p.G - head.row0)) return;
-    const int n = head.last - cta + 1;
-    auto part = [&](int i) { return part_of(p, ctas, D, cta + i, i == 0 ? 1 : 0); };
-    float m = -INFINITY;
-    for (int i = tid; i < n; i += THREADS) m = fmaxf(m, part(i)[row]);
+    for (int w = 0; w < WARPS; ++w) {
+        const int first = blockIdx.x * WARPS + w;
+        const Header head = reinterpret_cast<const Header *>(p.work)[first];
+        if (head.last < 0 || row >= min(ROWS, p.G - head.row0)) continue;
+        const int n = head.last - first + 1;
+        auto part = [&](int i) { return part_of(p, warps, D, first + i, i == 0 ? 1 : 0); };
+        float m = -INFINITY;
+        for (int i = tid; i < n; i += JOIN_THREADS) m = fmaxf(m, part(i)[row]);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if ((tid & 31) == 0) red[tid >> 5] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    const float mu = m == -INFINITY ? 0.f : m;
-    float l = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        if ((tid & 31) == 0) red[tid >> 5] = m;
+        __syncthreads();
+#pragma unroll
+        for (int x = 0; x < JOIN_WARPS; ++x) m = fmaxf(m, red[x]);
+        const float mu = m == -INFINITY ? 0.f : m;
+        float l = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-    for (int i = grp; i < n; i += GROUPS) {
-        const float *from = part(i);
-        const float f = ex2(from[row] - mu);
-        const float4 x = *reinterpret_cast<const float4 *>(from + 2 * ROWS + row * D + quad * 4);
-        l = fmaf(from[ROWS + row], f, l);
-        acc.x = fmaf(x.x, f, acc.x); acc.y = fmaf(x.y, f, acc.y);
-        acc.z = fmaf(x.z, f, acc.z); acc.w = fmaf(x.w, f, acc.w);
-    }
-    if (quad == 0) l_s[grp] = l;
-    acc_s[grp][quad] = acc;
-    __syncthreads();
-    if (grp > 0) return;
-    l = 0.f;
-    acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i = grp; i < n; i += GROUPS) {
+            const float *from = part(i);
+            const float f = ex2(from[row] - mu);
+            const float4 x = *reinterpret_cast<const float4 *>(from + 2 * ROWS + row * D + quad * 4);
+            l = fmaf(from[ROWS + row], f, l);
+            acc.x = fmaf(x.x, f, acc.x); acc.y = fmaf(x.y, f, acc.y);
+            acc.z = fmaf(x.z, f, acc.z); acc.w = fmaf(x.w, f, acc.w);
+        }
+        if (quad == 0) l_s[grp] = l;
+        acc_s[grp][quad] = acc;
+        __syncthreads();
+        if (grp == 0) {
+            l = 0.f;
+            acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int g = 0; g < GROUPS; ++g) {
-        const float4 x = acc_s[g][quad];
-        l += l_s[g];
-        acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w;
-    }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    const int h = head.hk * p.G + head.row0 + row;
-    T *out = reinterpret_cast<T *>(p.o) + (int64_t)head.b * p.o_sb + (int64_t)h * p.o_sh;
-    const float y[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
+            for (int g = 0; g < GROUPS; ++g) {
+                const float4 x = acc_s[g][quad];
+                l += l_s[g];
+                acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w;
+            }
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            const int h = head.hk * p.G + head.row0 + row;
+            T *out = reinterpret_cast<T *>(p.o) + (int64_t)head.b * p.o_sb + (int64_t)h * p.o_sh;
+            const float y[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-        if (quad * 4 + e < p.d) out[quad * 4 + e] = from_f32<T>(y[e]);
-    if (p.lse && quad == 0) p.lse[(int64_t)head.b * p.Hq + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
+            for (int e = 0; e < 4; ++e)
+                if (quad * 4 + e < p.d) out[quad * 4 + e] = from_f32<T>(y[e]);
+            if (p.lse && quad == 0) p.lse[(int64_t)head.b * p.Hq + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
+        }
+        __syncthreads();        // the next unit's parts go to the same shared memory
+    }
 }
 
-// CTAs of the grid: what the SMs hold at once, and no more than there can be tiles.
-int grid_size(int64_t B, int64_t units, int64_t max_keys, int resident) {
-    const int64_t most = B * units * ((max_keys + KEYS - 1) / KEYS);
+// CTAs of the grid: what the SMs hold at once, and no more than there can be runs.
+int grid_size(int64_t B, int64_t units, int64_t max_keys, int D, int resident) {
+    const int64_t most = B * units * (ceil_div64(max_keys, tile_keys(D)) + UNIT_COST);
     const int64_t room = (int64_t)num_sms() * resident;
-    const int64_t n = (most + MIN_TILES - 1) / MIN_TILES;
+    const int64_t n = ceil_div64(most, MIN_COST * WARPS);
     return (int)(n < 1 ? 1 : n < room ? n : room);
 }
 
 template <typename T, int D, bool VEC, bool BIAS>
 int launch(AttnParams &p, int64_t max_keys, cudaStream_t st) {
     auto kernel = attn_kernel<T, D, VEC, BIAS>;
-    const size_t smem = sizeof(Smem<T, D>) + (BIAS ? (size_t)p.borders.side * ROWS * sizeof(float) : 0);
-    // one opt-in per kernel, for the largest table: opting in to a smaller one would take a larger one back
-    const size_t largest = sizeof(Smem<T, D>) + (BIAS ? (size_t)relbias::MAX_SIDE * ROWS * sizeof(float) : 0);
-    if (int e = ensure_dyn_smem(reinterpret_cast<const void *>(kernel), largest)) return e;
-    const int fit = cached_occupancy(reinterpret_cast<const void *>(kernel), THREADS, smem);
-    const int grid = grid_size(p.B, p.units, max_keys, fit < ctas_per_sm(D) ? fit : ctas_per_sm(D));
+    constexpr size_t smem = sizeof(Smem<T, D>);
+    static_assert(CTAS_PER_SM * (smem + 1024) <= 228 << 10, "shared memory of an SM");
+    if (int e = ensure_dyn_smem(reinterpret_cast<const void *>(kernel), smem)) return e;
+    const int grid = grid_size(p.B, p.units, max_keys, D, CTAS_PER_SM);
     kernel<<<grid, THREADS, smem, st>>>(p);
     count_launch();
     if (int e = check_launch()) return e;
-    return sm100::launch_pdl(join_kernel<T, D>, dim3(grid, (unsigned)(p.G < ROWS ? p.G : ROWS)), THREADS, 0, st, p);
+    return sm100::launch_pdl(join_kernel<T, D>, dim3(grid, (unsigned)(p.G < ROWS ? p.G : ROWS)), JOIN_THREADS, 0, st, p);
 }
 template <typename T, int D>
 int launch(AttnParams &p, bool vec, int64_t max_keys, cudaStream_t st) {
@@ -558,7 +582,7 @@ extern "C" int64_t rgd_paged_attn_workspace_bytes(int64_t B, int64_t Hq, int64_t
     if (d > 128 || B > INT32_MAX || Hq > 65535 || max_pages > INT32_MAX || page_size > INT32_MAX) return RGD_E_SIZE;
     const int D = d > 64 ? 128 : 64;
     const int64_t units = Hkv * ceil_div64(Hq / Hkv, paged::ROWS);
-    return paged::workspace_bytes(paged::grid_size(B, units, max_pages * page_size, paged::ctas_per_sm(D)), D);
+    return paged::workspace_bytes(paged::grid_size(B, units, max_pages * page_size, D, paged::CTAS_PER_SM), D);
 }
 
 extern "C" int rgd_paged_attn(const rgd_heads *q, const rgd_paged *cache, const rgd_relbias *bias, const rgd_heads *o, float *lse,
