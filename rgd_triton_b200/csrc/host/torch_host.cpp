@@ -35,6 +35,7 @@
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/utils.h>
@@ -60,7 +61,8 @@ struct Api {
 #define RGD_FUNCTIONS(X)                                                                                              \
     X(device_supported) X(status_string) X(cache_create) X(cache_destroy) X(l2norm_fwd) X(l2norm_bwd) X(rmsnorm_fwd)   \
     X(rmsnorm_bwd) X(rmsnorm_bwd_workspace_bytes) X(headln_fwd) X(headln_bwd) X(rope) X(lnrope_fwd) X(lnrope_bwd)      \
-    X(attn_lse_rows) X(attn_fwd) X(attn_bwd) X(attn_bwd_workspace_bytes) X(attn_bwd_single_pass_workspace_bytes)
+    X(attn_lse_rows) X(attn_fwd) X(attn_bwd) X(attn_bwd_workspace_bytes) X(attn_bwd_single_pass_workspace_bytes)      \
+    X(relbias_fwd) X(relbias_bwd) X(relbias_bwd_workspace_bytes) X(paged_append) X(paged_attn) X(paged_attn_workspace_bytes)
     RGD_FUNCTIONS(RGD_FN)
 #undef RGD_FN
 };
@@ -796,6 +798,127 @@ PyObject *attn_call(Attn &a, const Tensor &q, const Tensor &k, const Tensor &v, 
     return return_lse ? wrap2(std::move(o), std::move(lse)) : THPVariable_Wrap(std::move(o));
 }
 
+// ------------------------------------------------------------------ learned relative position bias
+// weight, direction and the borders of its buckets (functional.relative_position_borders, a tuple)
+struct RelBias {
+    int64_t H = 0, buckets = 0;
+    int both = 0, dtype = 0;
+    std::vector<int32_t> borders;
+    rgd_relbias view(const Tensor &w) const { return {w.data_ptr(), w.stride(0), w.stride(1), dtype, (int)buckets, both, borders.data()}; }
+};
+
+bool relbias_ok(RelBias &r, const Tensor &w) {
+    if (!w.defined() || !w.is_cuda() || w.dim() != 2 || w.numel() == 0 || code_of(w) < 0 || special(w) || !device_ok(w.get_device()))
+        return false;
+    r.buckets = w.size(0);
+    r.H = w.size(1);
+    r.dtype = code_of(w);
+    return !(r.both && r.buckets % 2 != 0) && (int64_t)r.borders.size() + 1 == (r.both ? r.buckets / 2 : r.buckets);
+}
+
+bool borders_arg(PyObject *o, std::vector<int32_t> &out) {
+    if (!PyTuple_Check(o)) return false;
+    out.resize(PyTuple_GET_SIZE(o));
+    for (size_t i = 0; i < out.size(); ++i) {
+        const long v = PyLong_AsLong(PyTuple_GET_ITEM(o, i));
+        if (PyErr_Occurred() || v < 1 || v > INT32_MAX) {
+            PyErr_Clear();
+            return false;
+        }
+        out[i] = (int32_t)v;
+    }
+    return true;
+}
+
+struct RelBiasBackward : public Node {
+    RelBias r;
+    int64_t tq = 0, tk = 0, offset = 0, max_distance = 0;
+    at::TensorOptions weight_options, options;
+
+    std::string name() const override { return "RelativePositionBiasBackward"; }
+#define RGD_SAVED(f) (void)f;
+#define RGD_CONSTANTS(f) f(r.buckets, r.H, (bool)r.both, tq, tk, offset, max_distance, weight_options, options);
+    RGD_COMPILED(RGD_SAVED, RGD_CONSTANTS)
+#undef RGD_SAVED
+#undef RGD_CONSTANTS
+    variable_list apply(variable_list &&grads) override {
+        if (!grads[0].defined()) return {at::zeros({r.buckets, r.H}, weight_options)};
+        if (stand_in(grads[0])) {
+            const auto out = call_operator("rgd_b200::relbias_bwd", grads[0].contiguous(), r.buckets, (bool)r.both, max_distance, offset,
+                                           c10::typeMetaToScalarType(weight_options.dtype()));
+            return {out.at(0).toTensor()};
+        }
+        TORCH_CHECK(!at::GradMode::is_enabled() || !grads[0].requires_grad(), "RelativePositionBias has no second derivative");
+        const Tensor g = unit(grads[0]);
+        TORCH_CHECK(g.dim() == 4 && g.size(0) == 1 && g.size(1) == r.H && g.size(2) == tq && g.size(3) == tk && code_of(g) >= 0,
+                    "RelativePositionBias backward: the gradient does not match the bias");
+        c10::cuda::OptionalCUDAGuard guard(g.device());
+        at::AutoDispatchBelowADInplaceOrView below;
+        Tensor dw = new_buffer({r.buckets, r.H}, c10::typeMetaToScalarType(weight_options.dtype()), g.device());
+        const int64_t bytes = std::max<int64_t>(api.relbias_bwd_workspace_bytes(r.H, tq, tk, (int)r.buckets), 16);
+        Tensor work = new_buffer({bytes}, at::kByte, g.device());
+        const rgd_relbias b{nullptr, 0, 0, r.dtype, (int)r.buckets, r.both, r.borders.data()};
+        launched(api.relbias_bwd(&b, g.data_ptr(), g.stride(1), g.stride(2), code_of(g), dw.data_ptr(), r.H, tq, tk, offset,
+                                 work.data_ptr(), bytes, stream_of(g)), "relbias_bwd", false);
+        return {dw};
+    }
+};
+
+// rows that begin on 16 bytes, as the attention kernels stage them
+Tensor bias_rows(int64_t tq, int64_t tk, int64_t H, at::ScalarType type, c10::Device device) {
+    const int64_t ld = (tk + 7) / 8 * 8;
+    const int64_t sizes[4] = {1, H, tq, tk}, strides[4] = {H * tq * ld, tq * ld, ld, 1};
+    return at::detail::empty_strided_cuda(sizes, strides, type, device);
+}
+
+PyObject *relbias_call(RelBias &r, const Tensor &w, int64_t tq, int64_t tk, int64_t max_distance, int64_t offset, at::ScalarType type) {
+    Tensor out;
+    {
+        NoGil nogil;
+        c10::cuda::OptionalCUDAGuard guard(w.device());
+        out = bias_rows(tq, tk, r.H, type, w.device());
+        const rgd_relbias b = r.view(w);
+        launched(api.relbias_fwd(&b, out.data_ptr(), out.stride(1), out.stride(2), r.H, tq, tk, offset, code_of(out), stream_of(w)),
+                 "relbias_fwd", true);
+    }
+    if (wants_grad({&w})) {
+        auto node = new_node<RelBiasBackward>(torch::autograd::collect_next_edges(w));
+        node->r = std::move(r);
+        node->tq = tq;
+        node->tk = tk;
+        node->offset = offset;
+        node->max_distance = max_distance;
+        node->weight_options = w.options();
+        node->options = out.options();
+        torch::autograd::set_history(out, node);
+    }
+    return THPVariable_Wrap(std::move(out));
+}
+
+// ------------------------------------------------------------------ paged key-value cache
+bool ints(const Tensor &t, int64_t ndim, int64_t first, const Tensor &like) {
+    return t.defined() && t.scalar_type() == at::kInt && t.dim() == ndim && t.size(0) == first && t.device() == like.device() &&
+           !special(t) && t.numel() > 0 && t.stride(-1) == 1;
+}
+
+// A program's caches and tables; false: not covered here.
+bool paged_ok(rgd_paged &c, const Tensor &k, const Tensor &v, const Tensor &table, const Tensor &lengths, const Tensor &like, int64_t B,
+              int64_t heads) {
+    if (!plain(k, 4) || !plain(v, 4) || k.scalar_type() != like.scalar_type() || v.scalar_type() != like.scalar_type() ||
+        k.device() != like.device() || v.device() != like.device() || k.sizes() != v.sizes() || k.size(2) != heads ||
+        k.size(3) != like.size(3) || !ints(table, 2, B, like) || !ints(lengths, 1, B, like))
+        return false;
+    c = {k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), k.stride(2), v.stride(0), v.stride(1), v.stride(2),
+         k.size(0), k.size(1), table.data_ptr<int32_t>(), table.stride(0), table.size(1), lengths.data_ptr<int32_t>()};
+    return true;
+}
+
+bool half_type(const Tensor &t) { return t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16; }
+
+void written(const Tensor &t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // ------------------------------------------------------------------ Python entries
 // C++ exceptions become Python ones; an argument the library refuses hands the call back (None).  Saving a
 // tensor runs the user's pack hooks, and what those raise has to come out as it is: torch.utils.checkpoint
@@ -895,6 +1018,114 @@ PyObject *py_attn(PyObject *, PyObject *const *args, Py_ssize_t n) {
     });
 }
 
+// relbias(weight, borders, bidirectional, max_distance, seqlen_q, seqlen_k, offset, dtype): the caller has the borders of
+// these buckets and has checked the numbers
+PyObject *py_relbias(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    return guarded([&]() -> PyObject * {
+        RelBias r;
+        Tensor w;
+        if (n != 8 || !tensor_arg(args[0], w) || !THPDtype_Check(args[7]) || !borders_arg(args[1], r.borders)) Py_RETURN_NONE;
+        r.both = truth(args[2]) ? 1 : 0;
+        int64_t v[4];
+        for (int i = 0; i < 4; ++i) {
+            v[i] = PyLong_AsLongLong(args[3 + i]);
+            if (PyErr_Occurred()) return nullptr;
+        }
+        const at::ScalarType type = reinterpret_cast<THPDtype *>(args[7])->scalar_type;
+        if ((type != at::kFloat && type != at::kHalf && type != at::kBFloat16) || v[1] < 1 || v[2] < 1 || !relbias_ok(r, w)) Py_RETURN_NONE;
+        return relbias_call(r, w, v[1], v[2], v[0], v[3], type);
+    });
+}
+
+// paged_append(key, value, k_cache, v_cache, page_table, lengths, pos_emb or None, query or None, counts or None)
+// -> the rotated query, or False without one
+PyObject *py_paged_append(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    return guarded([&]() -> PyObject * {
+        Tensor key, value, kc, vc, table, lengths, pos, query, counts;
+        if (n != 9 || !tensor_arg(args[0], key) || !tensor_arg(args[1], value) || !tensor_arg(args[2], kc) || !tensor_arg(args[3], vc) ||
+            !tensor_arg(args[4], table) || !tensor_arg(args[5], lengths) || (args[6] != Py_None && !tensor_arg(args[6], pos)) ||
+            (args[7] != Py_None && !tensor_arg(args[7], query)) || (args[8] != Py_None && !tensor_arg(args[8], counts)))
+            Py_RETURN_NONE;
+        rgd_paged c;
+        if (!plain(key, 4) || !plain(value, 4) || !half_type(key) || !like(value, key) || value.sizes() != key.sizes() || key.size(3) > 128 ||
+            !device_ok(key.get_device()) || !paged_ok(c, kc, vc, table, lengths, key, key.size(0), key.size(2)))
+            Py_RETURN_NONE;
+        for (const Tensor *t : {&kc, &vc})
+            for (int i = 0; i < 3; ++i)
+                if (t->size(i) > 1 && t->stride(i) <= 0) Py_RETURN_NONE;
+        const int64_t B = key.size(0), N = key.size(1), Hkv = key.size(2), d = key.size(3);
+        int64_t P = 0, R = 0;
+        if (pos.defined()) {
+            if (!plain(pos, 3) || pos.size(0) != 2 || pos.device() != key.device() || pos.size(2) % 2 != 0 || pos.size(2) > d) Py_RETURN_NONE;
+            P = pos.size(1);
+            R = pos.size(2);
+        }
+        if (query.defined() && (!pos.defined() || !plain(query, 4) || !like(query, key) || query.size(0) != B || query.size(1) != N || query.size(3) != d))
+            Py_RETURN_NONE;
+        if ((counts.defined() && !ints(counts, 1, B, key)) || wants_grad({&key, &value, &kc, &vc, &pos, &query})) Py_RETURN_NONE;
+        Tensor out;
+        {
+            NoGil nogil;
+            c10::cuda::OptionalCUDAGuard guard(key.device());
+            if (query.defined()) out = new_like(query);
+            const rgd_heads kv = Attn::view(key), vv = Attn::view(value);
+            rgd_heads qv{}, ov{};
+            if (query.defined()) {
+                qv = Attn::view(query);
+                ov = Attn::view(out);
+            }
+            launched(api.paged_append(&kv, &vv, query.defined() ? &qv : nullptr, query.defined() ? &ov : nullptr, &c,
+                                      counts.defined() ? counts.data_ptr<int32_t>() : nullptr, pos.defined() ? pos.data_ptr() : nullptr,
+                                      pos.defined() ? pos.stride(0) : 0, pos.defined() ? pos.stride(1) : 0, P, R, B, N,
+                                      query.defined() ? query.size(2) : 0, Hkv, d, code_of(key), pos.defined() ? code_of(pos) : RGD_F32,
+                                      stream_of(key)), "paged_append", true);
+        }
+        written(kc);
+        written(vc);
+        if (!out.defined()) Py_RETURN_FALSE;
+        return THPVariable_Wrap(std::move(out));
+    });
+}
+
+// paged_attn(q, k_cache, v_cache, page_table, lengths, scale or None, weight or None, borders, bidirectional, return_lse)
+PyObject *py_paged_attn(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    return guarded([&]() -> PyObject * {
+        Tensor q, kc, vc, table, lengths, w;
+        if (n != 10 || !tensor_arg(args[0], q) || !tensor_arg(args[1], kc) || !tensor_arg(args[2], vc) || !tensor_arg(args[3], table) ||
+            !tensor_arg(args[4], lengths) || (args[6] != Py_None && !tensor_arg(args[6], w)))
+            Py_RETURN_NONE;
+        rgd_paged c;
+        if (!plain(q, 4) || !half_type(q) || q.size(1) != 1 || q.size(3) > 128 || !device_ok(q.get_device()) || !kc.defined() || kc.dim() != 4 ||
+            kc.size(2) < 1 || q.size(2) % kc.size(2) != 0 || !paged_ok(c, kc, vc, table, lengths, q, q.size(0), kc.size(2)) ||
+            wants_grad({&q, &kc, &vc, &w}))
+            Py_RETURN_NONE;
+        RelBias r;
+        if (w.defined()) {
+            r.both = truth(args[8]) ? 1 : 0;
+            if (!borders_arg(args[7], r.borders) || !relbias_ok(r, w) || w.device() != q.device() || r.H != q.size(2)) Py_RETURN_NONE;
+        }
+        const int64_t B = q.size(0), Hq = q.size(2), Hkv = kc.size(2), d = q.size(3);
+        const double scale = args[5] == Py_None ? 1.0 / sqrt((double)d) : PyFloat_AsDouble(args[5]);
+        if (PyErr_Occurred()) return nullptr;
+        const bool return_lse = truth(args[9]);
+        Tensor o, lse;
+        {
+            NoGil nogil;
+            c10::cuda::OptionalCUDAGuard guard(q.device());
+            o = new_like(q);
+            if (return_lse) lse = new_buffer({B, Hq}, at::kFloat, q.device());
+            const int64_t bytes = std::max<int64_t>(api.paged_attn_workspace_bytes(B, Hq, Hkv, d, c.max_pages, c.page_size), 16);
+            Tensor work = new_buffer({bytes}, at::kByte, q.device());
+            const rgd_heads qv = Attn::view(q), ov = Attn::view(o);
+            rgd_relbias b{};
+            if (w.defined()) b = r.view(w);
+            launched(api.paged_attn(&qv, &c, w.defined() ? &b : nullptr, &ov, return_lse ? lse.data_ptr<float>() : nullptr, B, Hq, Hkv, d,
+                                    (float)scale, code_of(q), work.data_ptr(), bytes, stream_of(q)), "paged_attn", true);
+        }
+        return return_lse ? wrap2(std::move(o), std::move(lse)) : THPVariable_Wrap(std::move(o));
+    });
+}
+
 PyObject *py_set_single_pass(PyObject *, PyObject *on) {
     single_pass.store(PyObject_IsTrue(on));
     Py_RETURN_NONE;
@@ -956,6 +1187,9 @@ PyMethodDef methods[] = {{"bind", py_bind, METH_O, "bind the C ABI of an opened 
                          {"headln", FAST(py_headln), "LayerNorm over head_dim of q and k"},
                          {"rotary", FAST(py_rotary), "rotary embedding of q and k, LayerNorm first when an eps is given"},
                          {"attn", FAST(py_attn), "attention"},
+                         {"relbias", FAST(py_relbias), "learned relative position bias"},
+                         {"paged_append", FAST(py_paged_append), "new keys and values into a paged cache"},
+                         {"paged_attn", FAST(py_paged_attn), "attention of one token over a paged cache"},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_host", "native host path of the operator set", -1, methods,
                           nullptr, nullptr, nullptr, nullptr};

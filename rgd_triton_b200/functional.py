@@ -51,6 +51,7 @@ import threading
 import weakref
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import Bias, Heads, Paged, RelBias, Rows
@@ -1101,6 +1102,14 @@ def _relbias_struct(weight, bidirectional: bool, max_distance: int, side: int) -
                    1 if bidirectional else 0, (C.c_int32 * len(borders))(*borders))
 
 
+def _borders_for(weight, bidirectional: bool, max_distance: int):
+    """The buckets' borders for the native path; None where the arguments are not what it covers."""
+    if weight.ndim != 2:
+        return None
+    side = weight.shape[0] // 2 if bidirectional else weight.shape[0]
+    return relative_position_borders(side, max_distance) if 2 <= side <= 256 and side // 2 < max_distance < 1 << 28 else None
+
+
 def _bias_rows(seqlen_q: int, seqlen_k: int, nheads: int, dtype, device):
     """(1, nheads, seqlen_q, seqlen_k) whose rows begin on 16 bytes, as the attention kernels stage them."""
     full = torch.empty((1, nheads, seqlen_q, (seqlen_k + 7) // 8 * 8), dtype=dtype, device=device)
@@ -1150,6 +1159,7 @@ class RelativePositionBiasFunc(torch.autograd.Function):
         return _relbias_forward(weight, seqlen_q, seqlen_k, bidirectional, max_distance, offset, dtype)
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, dbias):
         return _relbias_backward(dbias, *ctx.args), None, None, None, None, None, None
 
@@ -1165,6 +1175,14 @@ def relative_position_bias_fn(weight, seqlen_q, seqlen_k, bidirectional=True, ma
     of the result begin on 16 bytes whatever seqlen_k is (it may be a view of a wider tensor)."""
     seqlen_q, seqlen_k, offset, max_distance = int(seqlen_q), int(seqlen_k), int(offset), int(max_distance)
     bidirectional, dtype = bool(bidirectional), dtype or weight.dtype
+    if _tracing():
+        return torch.ops.rgd_b200.relbias(weight, seqlen_q, seqlen_k, bidirectional, max_distance, offset, dtype)
+    host = _HOST or _bind_host(weight)
+    if host is not None:
+        out = host.relbias(weight, _borders_for(weight, bidirectional, max_distance), bidirectional, max_distance, seqlen_q, seqlen_k,
+                           offset, dtype)
+        if out is not None:
+            return out
     if not _needs_grad(weight):
         return _relbias_forward(weight, seqlen_q, seqlen_k, bidirectional, max_distance, offset, dtype)
     return RelativePositionBiasFunc.apply(weight, seqlen_q, seqlen_k, bidirectional, max_distance, offset, dtype)
@@ -1201,6 +1219,8 @@ def _paged_struct(k_cache, v_cache, page_table, lengths) -> Paged:
 
 def _refuse_grad(what: str, *tensors) -> None:
     _require(not _needs_grad(*tensors), f"{what} has no backward pass: call it under torch.no_grad()")
+    if forward_ad._current_level >= 0:
+        _require(all(t is None or forward_ad.unpack_dual(t).tangent is None for t in tensors), f"{what} has no forward-mode derivative")
 
 
 def _written(*caches) -> None:
@@ -1275,6 +1295,14 @@ def paged_cache_append_fn(key, value, k_cache, v_cache, page_table, lengths, pos
     a token whose position has no page, or no row in pos_emb, is left out, and
     ``rgd_triton_b200._lib.load().rgd_device_status()`` reports it.  No two tokens of a call may map to the same slot.
     No backward pass."""
+    if _tracing():
+        out = torch.ops.rgd_b200.paged_append(key, value, k_cache, v_cache, page_table, lengths, pos_emb, query, counts)
+        return None if query is None else out
+    host = _HOST or _bind_host(key)
+    if host is not None:
+        out = host.paged_append(key, value, k_cache, v_cache, page_table, lengths, pos_emb, query, counts)
+        if out is not None:
+            return None if out is False else out
     _refuse_grad("paged_cache_append", key, value, query, k_cache, v_cache, pos_emb)
     out = _append_launch(key, value, k_cache, v_cache, page_table, lengths, pos_emb, query, counts)
     _written(k_cache, v_cache)
@@ -1326,7 +1354,17 @@ def paged_attention_func(q, k_cache, v_cache, page_table, lengths, softmax_scale
 
     Nothing is read back from the device: keys of pages outside the pool are left out, a length past the table's pages
     is cut there, and ``rgd_triton_b200._lib.load().rgd_device_status()`` reports both.  No backward pass."""
+    bidirectional, max_distance = bool(bidirectional), int(max_distance)
+    if _tracing():
+        o, lse = torch.ops.rgd_b200.paged_attn(q, k_cache, v_cache, page_table, lengths, softmax_scale, rel_weight, bidirectional, max_distance)
+        return (o, lse) if return_lse else o
+    host = _HOST or _bind_host(q)
+    if host is not None:
+        borders = None if rel_weight is None else _borders_for(rel_weight, bidirectional, max_distance)
+        out = host.paged_attn(q, k_cache, v_cache, page_table, lengths, softmax_scale, rel_weight, borders, bidirectional, return_lse)
+        if out is not None:
+            return out
     _refuse_grad("paged_attention", q, k_cache, v_cache, rel_weight)
     scale = 1.0 / math.sqrt(max(q.shape[-1], 1)) if softmax_scale is None else softmax_scale
-    o, lse = _paged_attn_launch(q, k_cache, v_cache, page_table, lengths, scale, rel_weight, bool(bidirectional), int(max_distance))
+    o, lse = _paged_attn_launch(q, k_cache, v_cache, page_table, lengths, scale, rel_weight, bidirectional, max_distance)
     return (o, lse) if return_lse else o

@@ -16,8 +16,14 @@ on this route (a compiled graph calls the operator directly).
     torch.ops.rgd_b200.rope(q, k, pos, cut_q, cut_k, heads_second, transposed) -> (qo, ko)
     torch.ops.rgd_b200.lnrope(q, k, pos, cut_q, cut_k, heads_second, eps) -> (qo, ko)
     torch.ops.rgd_b200.attn(q, k, v, bias, causal, softmax_scale) -> (o, lse)      (bias may require grad)
+    torch.ops.rgd_b200.relbias(weight, seqlen_q, seqlen_k, bidirectional, max_distance, offset, dtype) -> bias
 
-plus a ``*_bwd`` operator for each, which the autograd formulas call.
+plus a ``*_bwd`` operator for each, which the autograd formulas call, and without one
+
+    torch.ops.rgd_b200.paged_append(key, value, k_cache, v_cache, page_table, lengths, pos_emb, query, counts) -> query
+        (k_cache and v_cache are written; without a query the result is empty)
+    torch.ops.rgd_b200.paged_attn(q, k_cache, v_cache, page_table, lengths, softmax_scale, rel_weight, bidirectional,
+                                  max_distance) -> (o, lse)
 """
 from __future__ import annotations
 
@@ -236,3 +242,55 @@ def _attn_backward(ctx, do, dlse):
 
 
 attn.register_autograd(_attn_backward, setup_context=_attn_setup)
+
+
+# ----------------------------------------------------------------------------- position bias, paged cache
+@_op("rgd_b200::relbias", mutates_args=())
+def relbias(weight: Tensor, seqlen_q: int, seqlen_k: int, bidirectional: bool, max_distance: int, offset: int, dtype: torch.dtype) -> Tensor:
+    return F_._relbias_forward(weight, seqlen_q, seqlen_k, bidirectional, max_distance, offset, dtype)
+
+
+@_op("rgd_b200::relbias_bwd", mutates_args=())
+def relbias_bwd(dbias: Tensor, num_buckets: int, bidirectional: bool, max_distance: int, offset: int, wdtype: torch.dtype) -> Tensor:
+    return F_._relbias_backward(dbias, num_buckets, wdtype, bidirectional, max_distance, offset)
+
+
+relbias.register_fake(lambda weight, seqlen_q, seqlen_k, bidirectional, max_distance, offset, dtype:
+                      F_._bias_rows(seqlen_q, seqlen_k, weight.shape[1], dtype, weight.device))
+relbias_bwd.register_fake(lambda dbias, num_buckets, bidirectional, max_distance, offset, wdtype:
+                          dbias.new_empty((num_buckets, dbias.shape[1]), dtype=wdtype))
+
+
+def _relbias_setup(ctx, inputs, output):
+    weight, _, _, ctx.bidirectional, ctx.max_distance, ctx.offset, _ = inputs
+    ctx.buckets, ctx.wdtype = weight.shape[0], weight.dtype
+
+
+def _relbias_grad(ctx, dbias):
+    dw = torch.ops.rgd_b200.relbias_bwd(dbias, ctx.buckets, ctx.bidirectional, ctx.max_distance, ctx.offset, ctx.wdtype)
+    return dw, None, None, None, None, None, None
+
+
+relbias.register_autograd(_relbias_grad, setup_context=_relbias_setup)
+
+
+@_op("rgd_b200::paged_append", mutates_args=("k_cache", "v_cache"))
+def paged_append(key: Tensor, value: Tensor, k_cache: Tensor, v_cache: Tensor, page_table: Tensor, lengths: Tensor,
+                 pos_emb: Optional[Tensor], query: Optional[Tensor], counts: Optional[Tensor]) -> Tensor:
+    out = F_._append_launch(key, value, k_cache, v_cache, page_table, lengths, pos_emb, query, counts)
+    return key.new_empty(0) if out is None else out
+
+
+paged_append.register_fake(lambda key, value, k_cache, v_cache, page_table, lengths, pos_emb, query, counts:
+                           key.new_empty(0) if query is None else torch.empty_like(query))
+
+
+@_op("rgd_b200::paged_attn", mutates_args=())
+def paged_attn(q: Tensor, k_cache: Tensor, v_cache: Tensor, page_table: Tensor, lengths: Tensor, softmax_scale: Optional[float],
+               rel_weight: Optional[Tensor], bidirectional: bool, max_distance: int) -> Tuple[Tensor, Tensor]:
+    scale = q.shape[-1] ** -0.5 if softmax_scale is None else softmax_scale
+    return F_._paged_attn_launch(q, k_cache, v_cache, page_table, lengths, scale, rel_weight, bidirectional, max_distance)
+
+
+paged_attn.register_fake(lambda q, k_cache, v_cache, page_table, lengths, softmax_scale, rel_weight, bidirectional, max_distance:
+                         (torch.empty_like(q), q.new_empty((q.shape[0], q.shape[2]), dtype=torch.float32)))
