@@ -459,7 +459,8 @@ int64_t rgd_paged_attn_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv,
  * adds weight[bucket(lengths[b] - 1 - j), h].  lse (NULL or fp32 [B, Hq]):
  * log-sum-exp.  A sequence of length 0 gets zeros and lse -inf; so does one
  * without a usable page.  Keys of pages out of range are left out.  dtype
- * RGD_F16 / RGD_BF16, d <= 128, Hq a multiple of Hkv.  The order of all sums
+ * RGD_F16 / RGD_BF16, d <= 128, Hq a multiple of Hkv, B * Hkv * ceil(Hq / Hkv /
+ * 16) * (max_pages * page_size / 16 + 3) below 2^31.  The order of all sums
  * depends on the lengths and the device alone, not on the run. */
 int rgd_paged_attn(const rgd_heads *q, const rgd_paged *cache,
                    const rgd_relbias *bias, const rgd_heads *o, float *lse,

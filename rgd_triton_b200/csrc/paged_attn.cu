@@ -62,7 +62,7 @@ __device__ __forceinline__ int live_length(const AttnParams &p, int b, bool repo
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int WARPS = 4, THREADS = WARPS * 32, ROWS = 16, STAGES = 3, CTAS_PER_SM = 2;
 constexpr int UNIT_COST = 2;            // of a unit's queries and output, in tiles
-constexpr int MIN_COST = 6;             // least run of a warp
+constexpr int MIN_COST = 3;             // least run of a warp
 
 __host__ __device__ constexpr int tile_keys(int D) { return D > 64 ? 16 : 32; }      // 8 KB of keys and values
 
@@ -76,10 +76,9 @@ struct Smem {
     };
     Stage ring[WARPS][STAGES];
     int64_t row[WARPS][2][2 * KEYS];                    // of the tiles to load next: element offsets of keys, of values; -1: none
-    int64_t sums[WARPS];
-    int counts[WARPS];
+    int sums[WARPS], counts[WARPS];
     struct Boundary {                                   // where a warp's run begins
-        int64_t tiles;                                  // of all units before it
+        int tiles;                                      // of all units before it
         int b, unit, tile;
     } at[WARPS + 1];
     int borders[relbias::MAX_SIDE];                     // with a position bias
@@ -110,6 +109,21 @@ __device__ __forceinline__ float *part_of(const AttnParams &p, int warps, int D,
     return reinterpret_cast<float *>(p.work + (int64_t)warps * sizeof(Header)) + (warp * 2 + which) * part_floats(D);
 }
 
+// The costs [0, total) dealt out to the warps: equal shares, the first ones with one more.
+struct Runs {
+    int total, busy, share, more;       // busy: warps with a share
+    __device__ __forceinline__ Runs(int total, int warps) : total(total) {
+        busy = min(warps, (total + MIN_COST - 1) / MIN_COST);
+        share = busy > 0 ? total / busy : 0;
+        more = total - share * busy;
+    }
+    __device__ __forceinline__ int begin(int w) const { return w >= busy ? total : w * share + min(w, more); }
+    __device__ __forceinline__ int owner(int pos) const {
+        const int longer = more * (share + 1);
+        return pos < longer ? pos / (share + 1) : more + (pos - longer) / share;
+    }
+};
+
 // Where a warp stands in the tiles of all units.
 struct Cursor {
     int b, hk, group, tile, tiles, len;
@@ -130,19 +144,16 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attn_kernel(const __grid
 
     // cost of a head's units before each sequence: every thread sums a run of sequences, then the runs are added up
     const int chunk = (p.B + THREADS - 1) / THREADS, b0 = min(tid * chunk, p.B), b1 = min(b0 + chunk, p.B);
-    int64_t mine = 0, upto;
-    int filled = 0, filled_upto;                            // sequences with a token
+    int mine = 0, filled = 0;                               // cost; sequences with a token
     for (int b = b0; b < b1; ++b) {
         const int tiles = tiles_of(live_length(p, b, blockIdx.x == 0));
         mine += cost_of(tiles);
         filled += tiles > 0;
     }
-    upto = mine;
-    filled_upto = filled;
+    int upto = mine, filled_upto = filled;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
-        const int y = __shfl_up_sync(0xffffffffu, filled_upto, o);
+        const int x = __shfl_up_sync(0xffffffffu, upto, o), y = __shfl_up_sync(0xffffffffu, filled_upto, o);
         if (lane >= o) {
             upto += x;
             filled_upto += y;
@@ -155,7 +166,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attn_kernel(const __grid
     if (BIAS)
         for (int k = tid; k < p.borders.side - 1; k += THREADS) sm.borders[k] = p.borders.at[k];
     __syncthreads();
-    int64_t all = 0;
+    int all = 0;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) {
         if (w < warp) {
@@ -164,34 +175,30 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attn_kernel(const __grid
         }
         all += sm.sums[w];
     }
-    const int64_t total = all * p.units;
-    const int64_t busy = min((int64_t)warps, (total + MIN_COST - 1) / MIN_COST);       // warps with a run
+    const Runs runs(all * p.units, warps);
     // the boundaries of this CTA's runs: the thread whose sequences a boundary lies in finds it.  A unit's cost comes
     // before its tiles.
 #pragma unroll
     for (int w = 0; w <= WARPS; ++w) {
-        const int64_t first = min((int64_t)blockIdx.x * WARPS + w, busy);
-        const int64_t pos = busy > 0 ? first * total / busy : 0;
-        int64_t before = upto - mine;
-        int64_t filled_before = filled_upto - filled;
+        const int pos = runs.begin((int)blockIdx.x * WARPS + w);
+        int before = upto - mine, filled_before = filled_upto - filled;
         if (pos >= before * p.units && pos < upto * p.units) {
             for (int b = b0; b < b1; ++b) {
                 const int tiles = tiles_of(live_length(p, b, false)), cost = cost_of(tiles);
                 if (pos < (before + cost) * p.units) {
-                    const int64_t in = pos - before * p.units;
-                    const int unit = (int)(in / cost), tile = max((int)(in - (int64_t)unit * cost) - UNIT_COST, 0);
-                    sm.at[w] = {(before - filled_before * UNIT_COST) * p.units + (int64_t)unit * tiles + tile, b, unit, tile};
+                    const int in = pos - before * p.units, unit = in / cost, tile = max(in - unit * cost - UNIT_COST, 0);
+                    sm.at[w] = {(before - filled_before * UNIT_COST) * p.units + unit * tiles + tile, b, unit, tile};
                     break;
                 }
                 before += cost;
                 filled_before += tiles > 0;
             }
-        } else if (tid == THREADS - 1 && pos >= total) {
-            sm.at[w] = {(all - (int64_t)filled_upto * UNIT_COST) * p.units, p.B, 0, 0};
+        } else if (tid == THREADS - 1 && pos >= runs.total) {
+            sm.at[w] = {(all - filled_upto * UNIT_COST) * p.units, p.B, 0, 0};
         }
     }
     __syncthreads();
-    const int n = (int)(sm.at[warp + 1].tiles - sm.at[warp].tiles);
+    const int n = sm.at[warp + 1].tiles - sm.at[warp].tiles;
     if (lane == 0) reinterpret_cast<Header *>(p.work)[me].last = -1;
 
     Cursor at{}, to{};          // of the tile that is computed, of the tile whose table entries are fetched next
@@ -442,11 +449,9 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attn_kernel(const __grid
                 }
             }
             if (!done && whole && lane == 0) {
-                // The warp that has the unit's last tile: this run ends at cost position (me + 1) * total / busy, the
-                // unit as many tiles later as are left, and warp x's run is [x * total / busy, (x + 1) * total / busy).
-                const int64_t t = (me + 1) * total / busy - 1 + (at.tiles - 1 - at.tile);
+                // this run ends before the tiles that are left of the unit
                 Header &head = reinterpret_cast<Header *>(p.work)[me];
-                head.last = (int)(((t + 1) * busy - 1) / total);
+                head.last = runs.owner(runs.begin(me + 1) - 1 + (at.tiles - 1 - at.tile));
                 head.b = at.b;
                 head.hk = at.hk;
                 head.row0 = row0;
@@ -469,54 +474,77 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attn_kernel(const __grid
         }
 }
 
-constexpr int JOIN_THREADS = 256, JOIN_WARPS = JOIN_THREADS / 32;
+constexpr int JOIN_THREADS = 256;
 
 // Adds the parts of the units that begin in the runs of the attention's CTA blockIdx.x and end in other warps'; one CTA
 // per row.
 template <typename T, int D>
 __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const __grid_constant__ AttnParams p) {
     constexpr int QUADS = D / 4, GROUPS = JOIN_THREADS / QUADS;
-    __shared__ float red[JOIN_WARPS], l_s[GROUPS];
+    __shared__ float m_s[GROUPS], l_s[GROUPS];
     __shared__ float4 acc_s[GROUPS][QUADS];
     const int tid = threadIdx.x, quad = tid % QUADS, grp = tid / QUADS, row = blockIdx.y, warps = gridDim.x * WARPS;
     sm100::grid_wait();
+    Header heads[WARPS];
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) heads[w] = reinterpret_cast<const Header *>(p.work)[blockIdx.x * WARPS + w];
+#pragma unroll
     for (int w = 0; w < WARPS; ++w) {
+        const Header head = heads[w];
         const int first = blockIdx.x * WARPS + w;
-        const Header head = reinterpret_cast<const Header *>(p.work)[first];
         if (head.last < 0 || row >= min(ROWS, p.G - head.row0)) continue;
         const int n = head.last - first + 1;
-        auto part = [&](int i) { return part_of(p, warps, D, first + i, i == 0 ? 1 : 0); };
-        float m = -INFINITY;
-        for (int i = tid; i < n; i += JOIN_THREADS) m = fmaxf(m, part(i)[row]);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        if ((tid & 31) == 0) red[tid >> 5] = m;
-        __syncthreads();
-#pragma unroll
-        for (int x = 0; x < JOIN_WARPS; ++x) m = fmaxf(m, red[x]);
-        const float mu = m == -INFINITY ? 0.f : m;
-        float l = 0.f;
+        // each group of threads adds up every GROUPS-th part, four at a time; then the groups are added up in order
+        float m = -INFINITY, l = 0.f;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-        for (int i = grp; i < n; i += GROUPS) {
-            const float *from = part(i);
-            const float f = ex2(from[row] - mu);
-            const float4 x = *reinterpret_cast<const float4 *>(from + 2 * ROWS + row * D + quad * 4);
-            l = fmaf(from[ROWS + row], f, l);
-            acc.x = fmaf(x.x, f, acc.x); acc.y = fmaf(x.y, f, acc.y);
-            acc.z = fmaf(x.z, f, acc.z); acc.w = fmaf(x.w, f, acc.w);
+        for (int i0 = grp; i0 < n; i0 += 4 * GROUPS) {
+            float pm[4], pl[4];
+            float4 x[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int i = i0 + u * GROUPS;
+                pm[u] = -INFINITY;
+                pl[u] = 0.f;
+                x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (i < n) {
+                    const float *from = part_of(p, warps, D, first + i, i == 0 ? 1 : 0);
+                    pm[u] = from[row];
+                    pl[u] = from[ROWS + row];
+                    x[u] = *reinterpret_cast<const float4 *>(from + 2 * ROWS + row * D + quad * 4);
+                }
+            }
+            const float m_new = fmaxf(m, fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3])));
+            const float mu = m_new == -INFINITY ? 0.f : m_new, keep = ex2(m - mu);
+            l *= keep;
+            acc.x *= keep; acc.y *= keep; acc.z *= keep; acc.w *= keep;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const float f = ex2(pm[u] - mu);
+                l = fmaf(pl[u], f, l);
+                acc.x = fmaf(x[u].x, f, acc.x); acc.y = fmaf(x[u].y, f, acc.y);
+                acc.z = fmaf(x[u].z, f, acc.z); acc.w = fmaf(x[u].w, f, acc.w);
+            }
+            m = m_new;
         }
-        if (quad == 0) l_s[grp] = l;
+        if (quad == 0) {
+            m_s[grp] = m;
+            l_s[grp] = l;
+        }
         acc_s[grp][quad] = acc;
         __syncthreads();
         if (grp == 0) {
+#pragma unroll
+            for (int g = 0; g < GROUPS; ++g) m = fmaxf(m, m_s[g]);
+            const float mu = m == -INFINITY ? 0.f : m;
             l = 0.f;
             acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int g = 0; g < GROUPS; ++g) {
                 const float4 x = acc_s[g][quad];
-                l += l_s[g];
-                acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w;
+                const float f = ex2(m_s[g] - mu);
+                l = fmaf(l_s[g], f, l);
+                acc.x = fmaf(x.x, f, acc.x); acc.y = fmaf(x.y, f, acc.y);
+                acc.z = fmaf(x.z, f, acc.z); acc.w = fmaf(x.w, f, acc.w);
             }
             const float inv = l == 0.f ? 0.f : 1.f / l;
             const int h = head.hk * p.G + head.row0 + row;
@@ -529,6 +557,11 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const __grid_constan
         }
         __syncthreads();        // the next unit's parts go to the same shared memory
     }
+}
+
+// Costs are 32-bit.
+bool too_large(int64_t B, int64_t units, int64_t max_keys, int D) {
+    return (double)B * (double)units * (double)(ceil_div64(max_keys, tile_keys(D)) + UNIT_COST) > (double)INT32_MAX;
 }
 
 // CTAs of the grid: what the SMs hold at once, and no more than there can be runs.
@@ -582,6 +615,7 @@ extern "C" int64_t rgd_paged_attn_workspace_bytes(int64_t B, int64_t Hq, int64_t
     if (d > 128 || B > INT32_MAX || Hq > 65535 || max_pages > INT32_MAX || page_size > INT32_MAX) return RGD_E_SIZE;
     const int D = d > 64 ? 128 : 64;
     const int64_t units = Hkv * ceil_div64(Hq / Hkv, paged::ROWS);
+    if (paged::too_large(B, units, max_pages * page_size, D)) return RGD_E_SIZE;
     return paged::workspace_bytes(paged::grid_size(B, units, max_pages * page_size, D, paged::CTAS_PER_SM), D);
 }
 
@@ -615,8 +649,9 @@ extern "C" int rgd_paged_attn(const rgd_heads *q, const rgd_paged *cache, const 
     p.groups = (p.G + paged::ROWS - 1) / paged::ROWS;
     p.units = p.Hkv * p.groups;
     const int64_t max_keys = cache->max_pages * cache->page_size;
-    if (workspace_bytes < rgd_paged_attn_workspace_bytes(B, Hq, Hkv, d, cache->max_pages, cache->page_size) || !workspace)
-        return RGD_E_WORKSPACE;
+    const int64_t need = rgd_paged_attn_workspace_bytes(B, Hq, Hkv, d, cache->max_pages, cache->page_size);
+    if (need < 0) return (int)need;
+    if (workspace_bytes < need || !workspace) return RGD_E_WORKSPACE;
     if (!is_aligned(workspace, 16)) return RGD_E_STRIDE;
     p.work = reinterpret_cast<char *>(workspace);
     const bool vec = d % 8 == 0 && paged::cache_vec16(*cache) && paged::heads_vec16(*q) && paged::heads_vec16(*o);
