@@ -63,6 +63,7 @@ __device__ __forceinline__ int live_length(const AttnParams &p, int b, bool repo
 constexpr int WARPS = 4, THREADS = WARPS * 32, ROWS = 16, STAGES = 3, CTAS_PER_SM = 2;
 constexpr int UNIT_COST = 2;            // of a unit's queries and output, in tiles
 constexpr int MIN_COST = 3;             // least run of a warp
+static_assert(MIN_COST > UNIT_COST, "a run that begins a unit has its first tile");
 
 __host__ __device__ constexpr int tile_keys(int D) { return D > 64 ? 16 : 32; }      // 8 KB of keys and values
 
@@ -98,10 +99,13 @@ __device__ __forceinline__ float ex2(float x) {
 // Workspace: per warp of the grid a header and two parts, [0] of a unit that began in another warp's run, [1] of one
 // that ends in another's.
 struct Header {
-    int last;                   // the unit of part [1] ends in this warp; -1: there is none
+    int last;                   // the unit of part [1] ends in this warp's run; -1: there is none
+    int merged;                 // part [1] holds what the four warps of the CTA have
     int b, hk, row0;
 };
-__host__ __device__ __forceinline__ int64_t part_floats(int D) { return ROWS * (D + 2); }
+// A CTA whose runs lie inside one unit that ends behind them leaves one part, its first warp's.  So of a unit that ends
+// in another CTA, every CTA in between has one part, the last one a part per warp, the first one either.
+__host__ __device__ constexpr int64_t part_floats(int D) { return ROWS * (D + 2); }
 __host__ __device__ __forceinline__ int64_t workspace_bytes(int ctas, int D) {
     return (int64_t)ctas * WARPS * ((int64_t)sizeof(Header) + 2 * part_floats(D) * (int64_t)sizeof(float));
 }
@@ -113,7 +117,7 @@ __device__ __forceinline__ float *part_of(const AttnParams &p, int warps, int D,
 struct Runs {
     int total, busy, share, more;       // busy: warps with a share
     __device__ __forceinline__ Runs(int total, int warps) : total(total) {
-        busy = min(warps, (total + MIN_COST - 1) / MIN_COST);
+        busy = total == 0 ? 0 : max(1, min(warps, total / MIN_COST));       // a share is at least MIN_COST: a tile
         share = busy > 0 ? total / busy : 0;
         more = total - share * busy;
     }
@@ -200,6 +204,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attn_kernel(const __grid
     __syncthreads();
     const int n = sm.at[warp + 1].tiles - sm.at[warp].tiles;
     if (lane == 0) reinterpret_cast<Header *>(p.work)[me].last = -1;
+    const bool merge = sm.at[0].b < p.B && sm.at[0].b == sm.at[WARPS].b && sm.at[0].unit == sm.at[WARPS].unit;
 
     Cursor at{}, to{};          // of the tile that is computed, of the tile whose table entries are fetched next
     if (n > 0) {
@@ -322,6 +327,19 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attn_kernel(const __grid
             m_ref[0] = m_ref[1] = -INFINITY;
             l_sum[0] = l_sum[1] = 0.f;
         }
+        float add[BIAS ? KT : 1][4];    // the position bias, read while the tile is on its way
+        if constexpr (BIAS) {
+            const int bucket = relbias::bucket_of_distance(sm.borders, p.borders.side, max(at.len - 1 - (at.tile * KEYS + my_key), 0));
+#pragma unroll
+            for (int t = 0; t < KT; ++t)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int64_t w_at = __shfl_sync(0xffffffffu, bucket, t * 8 + tq * 2 + e) * p.w_sk + (h0 + gq) * p.w_sh;
+#pragma unroll
+                    for (int r = 0; r < 2; ++r)
+                        add[t][r * 2 + e] = gq + r * 8 < rows ? load_as_f32(p.w, w_at + r * 8 * p.w_sh, p.w_dtype) : 0.f;
+                }
+        }
         asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
         __syncwarp();                   // this tile has landed; all lanes are done with the tile before it
         if (i + STAGES - 1 < n) load(i + STAGES - 1);
@@ -346,21 +364,16 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attn_kernel(const __grid
                 attn::Mma<T>::mma(s[t], aq[kk], bf[0], bf[1]);
                 attn::Mma<T>::mma(s[t + 1], aq[kk], bf[2], bf[3]);
             }
-        int bucket = 0;
-        if constexpr (BIAS) bucket = relbias::bucket_of_distance(sm.borders, p.borders.side, max(at.len - 1 - (at.tile * KEYS + my_key), 0));
         float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
         for (int t = 0; t < KT; ++t)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int key = t * 8 + tq * 2 + e;
-                int64_t w_at = 0;
-                if constexpr (BIAS) w_at = __shfl_sync(0xffffffffu, bucket, key) * p.w_sk + (h0 + gq) * p.w_sh;
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
                     float x = s[t][r * 2 + e] * p.scale_log2;
-                    if constexpr (BIAS)
-                        if (gq + r * 8 < rows) x += attn::bias_log2<float>(load_as_f32(p.w, w_at + r * 8 * p.w_sh, p.w_dtype));
+                    if constexpr (BIAS) x += attn::bias_log2<float>(add[t][r * 2 + e]);
                     if (!(live[0] >> key & 1)) x = -INFINITY;
                     s[t][r * 2 + e] = x;
                     mx[r] = fmaxf(mx[r], x);
@@ -437,7 +450,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attn_kernel(const __grid
                     }
                     if (p.lse && tq == 0)
                         p.lse[(int64_t)at.b * p.Hq + h0 + row] = l_sum[r] == 0.f ? -INFINITY : (m_ref[r] + log2f(l_sum[r])) * LN2;
-                } else {
+                } else if (!merge) {
                     float *part = part_of(p, warps, D, me, whole ? 1 : 0);
                     if (tq == 0) {
                         part[row] = m_ref[r];
@@ -452,6 +465,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attn_kernel(const __grid
                 // this run ends before the tiles that are left of the unit
                 Header &head = reinterpret_cast<Header *>(p.work)[me];
                 head.last = runs.owner(runs.begin(me + 1) - 1 + (at.tiles - 1 - at.tile));
+                head.merged = merge;
                 head.b = at.b;
                 head.hk = at.hk;
                 head.row0 = row0;
@@ -460,6 +474,51 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attn_kernel(const __grid
         advance(at);
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
+
+    if (merge) {                // uniform over the CTA; the rings are done with
+        const typename S::Boundary begins = sm.at[0];
+        const int hk = begins.unit / p.groups, rows = min(ROWS, p.G - (begins.unit - hk * p.groups) * ROWS);
+        float *mine_o = reinterpret_cast<float *>(sm.ring[warp]), *mine_m = mine_o + ROWS * D;       // then the sums
+        static_assert(sizeof(sm.ring[0]) >= part_floats(D) * sizeof(float), "a part in a warp's ring");
+        __syncwarp();
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const int row = gq + r * 8;
+            if (tq == 0) {
+                mine_m[row] = m_ref[r];
+                mine_m[ROWS + row] = l_sum[r];
+            }
+#pragma unroll
+            for (int j = 0; j < NT; ++j) *reinterpret_cast<float2 *>(mine_o + row * D + j * 8 + tq * 2) = make_float2(o[j][2 * r], o[j][2 * r + 1]);
+        }
+        __syncthreads();
+        float *part = part_of(p, warps, D, blockIdx.x * WARPS, begins.tile == 0 ? 1 : 0);
+        for (int e = tid; e < rows * (D / 4); e += THREADS) {
+            const int row = e / (D / 4), c = e % (D / 4) * 4;
+            const float *from[WARPS];
+            float m = -INFINITY, l = 0.f;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) {
+                from[w] = reinterpret_cast<const float *>(sm.ring[w]);
+                m = fmaxf(m, from[w][ROWS * D + row]);
+            }
+            const float mu = m == -INFINITY ? 0.f : m;
+            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) {
+                const float f = ex2(from[w][ROWS * D + row] - mu);
+                const float4 x = *reinterpret_cast<const float4 *>(from[w] + row * D + c);
+                l = fmaf(from[w][ROWS * D + ROWS + row], f, l);
+                y.x = fmaf(x.x, f, y.x); y.y = fmaf(x.y, f, y.y);
+                y.z = fmaf(x.z, f, y.z); y.w = fmaf(x.w, f, y.w);
+            }
+            *reinterpret_cast<float4 *>(part + 2 * ROWS + row * D + c) = y;
+            if (c == 0) {
+                part[row] = m;
+                part[ROWS + row] = l;
+            }
+        }
+    }
 
     // sequences without a token
     for (int b = blockIdx.x; b < p.B; b += gridDim.x)
@@ -493,7 +552,10 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const __grid_constan
         const Header head = heads[w];
         const int first = blockIdx.x * WARPS + w;
         if (head.last < 0 || row >= min(ROWS, p.G - head.row0)) continue;
-        const int n = head.last - first + 1;
+        // parts: of the first CTA, of the ones in between, of the last one
+        const int cta0 = blockIdx.x, cta1 = head.last / WARPS;
+        const int n0 = cta0 == cta1 ? head.last - first + 1 : head.merged ? 1 : WARPS - w;
+        const int n1 = max(cta1 - cta0 - 1, 0), n = n0 + n1 + (cta0 == cta1 ? 0 : head.last % WARPS + 1);
         // each group of threads adds up every GROUPS-th part, four at a time; then the groups are added up in order
         float m = -INFINITY, l = 0.f;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -507,7 +569,8 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const __grid_constan
                 pl[u] = 0.f;
                 x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
                 if (i < n) {
-                    const float *from = part_of(p, warps, D, first + i, i == 0 ? 1 : 0);
+                    const int of = i < n0 ? first + i : i < n0 + n1 ? (cta0 + 1 + i - n0) * WARPS : cta1 * WARPS + i - n0 - n1;
+                    const float *from = part_of(p, warps, D, of, i == 0 ? 1 : 0);
                     pm[u] = from[row];
                     pl[u] = from[ROWS + row];
                     x[u] = *reinterpret_cast<const float4 *>(from + 2 * ROWS + row * D + quad * 4);
