@@ -118,7 +118,7 @@ struct Runs {
     int total, busy, share, more;       // busy: warps with a share
     __device__ __forceinline__ Runs(int total, int warps) : total(total) {
         busy = total == 0 ? 0 : max(1, min(warps, total / MIN_COST));       // a share is at least MIN_COST: a tile
-        share = busy > 0 ? total / busy : 0;
+        share = busy > 0 ? (int)((unsigned)total / (unsigned)busy) : 0;
         more = total - share * busy;
     }
     __device__ __forceinline__ int begin(int w) const { return w >= busy ? total : w * share + min(w, more); }
@@ -190,7 +190,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attn_kernel(const __grid
             for (int b = b0; b < b1; ++b) {
                 const int tiles = tiles_of(live_length(p, b, false)), cost = cost_of(tiles);
                 if (pos < (before + cost) * p.units) {
-                    const int in = pos - before * p.units, unit = in / cost, tile = max(in - unit * cost - UNIT_COST, 0);
+                    const int in = pos - before * p.units, unit = (int)((unsigned)in / (unsigned)cost), tile = max(in - unit * cost - UNIT_COST, 0);
                     sm.at[w] = {(before - filled_before * UNIT_COST) * p.units + unit * tiles + tile, b, unit, tile};
                     break;
                 }
@@ -212,7 +212,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attn_kernel(const __grid
         at.len = live_length(p, at.b, false);
         at.tiles = tiles_of(at.len);
         at.tile = sm.at[warp].tile;
-        at.hk = sm.at[warp].unit / p.groups;
+        at.hk = (int)((unsigned)sm.at[warp].unit / (unsigned)p.groups);
         at.group = sm.at[warp].unit - at.hk * p.groups;
         to = at;
     }
@@ -234,28 +234,28 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attn_kernel(const __grid
     // (of keys and of values; of one of them where there are 16 keys) lies and leaves that in shared memory, and then
     // all lanes copy the rows, 16 bytes each.
     const int my_key = lane % KEYS;
-    int entry = -1, slot = 0, entry_hk = 0;     // fetched; entry -1: nothing to read
+    struct Fetched {
+        int entry, slot, hk;        // entry -1: nothing to read
+    };
     uint32_t live[STAGES + 1] = {};             // which of the keys of tile i, i + 1, ... there are
     auto fetch = [&]() {
+        Fetched f{-1, 0, to.hk};
         const int key = to.tile * KEYS + my_key;
-        entry = -1;
-        entry_hk = to.hk;
         if (key < to.len) {
             int index;
-            split_position(p.view, (uint32_t)key, index, slot);
-            entry = p.view.table[(int64_t)to.b * p.view.table_stride + index];
-            if (!page_ok(p.view, entry)) {
-                entry = -1;
-                g_attn_status = 1;
-            }
+            split_position(p.view, (uint32_t)key, index, f.slot);
+            f.entry = p.view.table[(int64_t)to.b * p.view.table_stride + index];
         }
         advance(to);
+        return f;
     };
-    auto find = [&](int i) {
-        if (KEYS == 32 || lane < KEYS) sm.row[warp][i & 1][lane] = entry < 0 ? -1 : entry * p.k_sp + slot * p.k_ss + entry_hk * p.k_sh;
+    auto find = [&](const Fetched &f, int i) {
+        const bool ok = page_ok(p.view, f.entry);
+        if (f.entry != -1 && !ok) g_attn_status = 1;
+        if (KEYS == 32 || lane < KEYS) sm.row[warp][i & 1][lane] = ok ? f.entry * p.k_sp + f.slot * p.k_ss + f.hk * p.k_sh : -1;
         if (KEYS == 32 || lane >= KEYS)
-            sm.row[warp][i & 1][KEYS + my_key] = entry < 0 ? -1 : entry * p.v_sp + slot * p.v_ss + entry_hk * p.v_sh;
-        return __ballot_sync(0xffffffffu, entry >= 0);
+            sm.row[warp][i & 1][KEYS + my_key] = ok ? f.entry * p.v_sp + f.slot * p.v_ss + f.hk * p.v_sh : -1;
+        return __ballot_sync(0xffffffffu, ok);
     };
     auto load = [&](int i) {
         typename S::Stage &st = sm.ring[warp][i % STAGES];
@@ -280,46 +280,58 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attn_kernel(const __grid
             }
         }
     };
-    static_assert(STAGES == 3, "the steps below are three tiles long");
-#pragma unroll
-    for (int i = 0; i < STAGES; ++i) {
-        if (i < n) {
-            fetch();
-            __syncwarp();
-            live[i] = find(i);
-            __syncwarp();
-            if (i < STAGES - 1) load(i);
-        }
-        if (i < STAGES - 1) asm volatile("cp.async.commit_group;" ::: "memory");
-    }
-    if (STAGES < n) fetch();
-
     uint32_t aq[D / 16][4];             // the unit's queries as A fragments, rows past the group and channels past d as zeros
     float o[NT][4];                     // rows gq and gq + 8
     float m_ref[2], l_sum[2];
     bool whole = false;                 // the unit's first tile was in this run
     const int mi = lane >> 3, mr = lane & 7;
 
+    auto read_queries = [&]() {
+        const int row0 = at.group * ROWS, rows = min(ROWS, p.G - row0);
+        const T *qg = reinterpret_cast<const T *>(p.q) + (int64_t)at.b * p.q_sb + (int64_t)(at.hk * p.G + row0) * p.q_sh;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int r = gq + (e & 1) * 8, c = kk * 16 + (e >> 1) * 8 + tq * 2;
+                uint32_t x = 0u;
+                if constexpr (VEC) {
+                    if (r < rows && c < p.d) x = *reinterpret_cast<const uint32_t *>(qg + (int64_t)r * p.q_sh + c);
+                } else if (r < rows) {
+                    const T *qr = qg + (int64_t)r * p.q_sh + c;
+                    x = attn::Mma<T>::pack(c < p.d ? to_f32<T>(qr[0]) : 0.f, c + 1 < p.d ? to_f32<T>(qr[1]) : 0.f);
+                }
+                aq[kk][e] = x;
+            }
+    };
+
+    static_assert(STAGES == 3, "the steps below are three tiles long");
+    Fetched next{-1, 0, 0};             // of tile i + STAGES once tile i is computed
+    if (n > 0) {
+        Fetched f[STAGES];              // the first tiles' entries together: one wait
+#pragma unroll
+        for (int i = 0; i < STAGES; ++i)
+            if (i < n) f[i] = fetch();
+        if (STAGES < n) next = fetch();
+        read_queries();
+#pragma unroll
+        for (int i = 0; i < STAGES; ++i) {
+            if (i < n) {
+                live[i] = find(f[i], i);
+                __syncwarp();
+                if (i < STAGES - 1) load(i);
+                __syncwarp();           // the third tile's rows go where the first one's were
+            }
+            if (i < STAGES - 1) asm volatile("cp.async.commit_group;" ::: "memory");
+        }
+    }
+
     for (int i = 0; i < n; ++i) {
         const int row0 = at.group * ROWS, rows = min(ROWS, p.G - row0);
         const int h0 = at.hk * p.G + row0;              // query head of row 0
         if (i == 0 || at.tile == 0) {
             whole = at.tile == 0;
-            const T *qg = reinterpret_cast<const T *>(p.q) + (int64_t)at.b * p.q_sb + (int64_t)h0 * p.q_sh;
-#pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int r = gq + (e & 1) * 8, c = kk * 16 + (e >> 1) * 8 + tq * 2;
-                    uint32_t x = 0u;
-                    if constexpr (VEC) {
-                        if (r < rows && c < p.d) x = *reinterpret_cast<const uint32_t *>(qg + (int64_t)r * p.q_sh + c);
-                    } else if (r < rows) {
-                        const T *qr = qg + (int64_t)r * p.q_sh + c;
-                        x = attn::Mma<T>::pack(c < p.d ? to_f32<T>(qr[0]) : 0.f, c + 1 < p.d ? to_f32<T>(qr[1]) : 0.f);
-                    }
-                    aq[kk][e] = x;
-                }
+            if (i > 0) read_queries();
 #pragma unroll
             for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -345,8 +357,8 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attn_kernel(const __grid
         if (i + STAGES - 1 < n) load(i + STAGES - 1);
         asm volatile("cp.async.commit_group;" ::: "memory");
         if (i + STAGES < n) {
-            live[STAGES] = find(i + STAGES);
-            if (i + STAGES + 1 < n) fetch();
+            live[STAGES] = find(next, i + STAGES);
+            if (i + STAGES + 1 < n) next = fetch();
         }
         const typename S::Stage &st = sm.ring[warp][i % STAGES];
 
@@ -533,10 +545,79 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attn_kernel(const __grid
         }
 }
 
-constexpr int JOIN_THREADS = 256;
+constexpr int JOIN_THREADS = WARPS * 32;
+constexpr int JOIN_FEW = 8;             // parts that one warp adds up by itself
+
+// The parts of a unit: of its first CTA, of the ones in between, of the last one.
+struct Parts {
+    int first, cta0, cta1, n0, n1, n;
+    __device__ __forceinline__ Parts(const Header &head, int first) : first(first), cta0(first / WARPS), cta1(head.last / WARPS) {
+        const bool one = cta0 == cta1;
+        n0 = one ? head.last - first + 1 : head.merged ? 1 : WARPS - first % WARPS;
+        n1 = max(cta1 - cta0 - 1, 0);
+        n = n0 + n1 + (one ? 0 : head.last % WARPS + 1);
+    }
+    __device__ __forceinline__ int warp(int i) const {
+        return i < n0 ? first + i : i < n0 + n1 ? (cta0 + 1 + i - n0) * WARPS : cta1 * WARPS + i - n0 - n1;
+    }
+};
+// A row's maximum, sum and four channels of its output, so far.
+struct Joined {
+    float m = -INFINITY, l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    __device__ __forceinline__ void rescale(float m_new) {
+        const float f = ex2(m - (m_new == -INFINITY ? 0.f : m_new));
+        l *= f;
+        acc.x *= f; acc.y *= f; acc.z *= f; acc.w *= f;
+        m = m_new;
+    }
+    __device__ __forceinline__ void add(float pm, float pl, const float4 &x) {          // pm <= m
+        const float f = ex2(pm - (m == -INFINITY ? 0.f : m));
+        l = fmaf(pl, f, l);
+        acc.x = fmaf(x.x, f, acc.x); acc.y = fmaf(x.y, f, acc.y);
+        acc.z = fmaf(x.z, f, acc.z); acc.w = fmaf(x.w, f, acc.w);
+    }
+    // parts i0, i0 + step, ..., U at a time
+    template <int U>
+    __device__ __forceinline__ void add_parts(const AttnParams &p, int warps, int D, const Parts &parts, int row, int quad, int i0, int step) {
+        for (; i0 < parts.n; i0 += U * step) {
+            float pm[U], pl[U], m_new = m;
+            float4 x[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int i = i0 + u * step;
+                pm[u] = -INFINITY;
+                pl[u] = 0.f;
+                x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (i < parts.n) {
+                    const float *from = part_of(p, warps, D, parts.warp(i), i == 0 ? 1 : 0);
+                    pm[u] = from[row];
+                    pl[u] = from[ROWS + row];
+                    x[u] = *reinterpret_cast<const float4 *>(from + 2 * ROWS + row * D + quad * 4);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) m_new = fmaxf(m_new, pm[u]);
+            rescale(m_new);
+#pragma unroll
+            for (int u = 0; u < U; ++u) add(pm[u], pl[u], x[u]);
+        }
+    }
+    template <typename T>
+    __device__ __forceinline__ void store(const AttnParams &p, const Header &head, int row, int quad) const {
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const int h = head.hk * p.G + head.row0 + row;
+        T *out = reinterpret_cast<T *>(p.o) + (int64_t)head.b * p.o_sb + (int64_t)h * p.o_sh;
+        const float y[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (quad * 4 + e < p.d) out[quad * 4 + e] = from_f32<T>(y[e]);
+        if (p.lse && quad == 0) p.lse[(int64_t)head.b * p.Hq + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
+    }
+};
 
 // Adds the parts of the units that begin in the runs of the attention's CTA blockIdx.x and end in other warps'; one CTA
-// per row.
+// per row.  Units of few parts are a warp's, one each; the others are taken by the CTA, one after another.
 template <typename T, int D>
 __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const __grid_constant__ AttnParams p) {
     constexpr int QUADS = D / 4, GROUPS = JOIN_THREADS / QUADS;
@@ -544,81 +625,43 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const __grid_constan
     __shared__ float4 acc_s[GROUPS][QUADS];
     const int tid = threadIdx.x, quad = tid % QUADS, grp = tid / QUADS, row = blockIdx.y, warps = gridDim.x * WARPS;
     sm100::grid_wait();
-    Header heads[WARPS];
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) heads[w] = reinterpret_cast<const Header *>(p.work)[blockIdx.x * WARPS + w];
-#pragma unroll
+    const Header *heads = reinterpret_cast<const Header *>(p.work) + blockIdx.x * WARPS;
+    auto there = [&](const Header &head) { return head.last >= 0 && row < min(ROWS, p.G - head.row0); };
+    bool many = false;
+    const Header mine = heads[tid / 32];
+    if (there(mine)) {
+        const Parts parts(mine, blockIdx.x * WARPS + tid / 32);
+        many = parts.n > JOIN_FEW;
+        if (!many && tid % 32 < QUADS) {
+            Joined sum;
+            sum.add_parts<JOIN_FEW>(p, warps, D, parts, row, tid % 32, 0, 1);
+            sum.store<T>(p, mine, row, tid % 32);
+        }
+    }
+    if (!__syncthreads_or(many)) return;
     for (int w = 0; w < WARPS; ++w) {
         const Header head = heads[w];
-        const int first = blockIdx.x * WARPS + w;
-        if (head.last < 0 || row >= min(ROWS, p.G - head.row0)) continue;
-        // parts: of the first CTA, of the ones in between, of the last one
-        const int cta0 = blockIdx.x, cta1 = head.last / WARPS;
-        const int n0 = cta0 == cta1 ? head.last - first + 1 : head.merged ? 1 : WARPS - w;
-        const int n1 = max(cta1 - cta0 - 1, 0), n = n0 + n1 + (cta0 == cta1 ? 0 : head.last % WARPS + 1);
-        // each group of threads adds up every GROUPS-th part, four at a time; then the groups are added up in order
-        float m = -INFINITY, l = 0.f;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int i0 = grp; i0 < n; i0 += 4 * GROUPS) {
-            float pm[4], pl[4];
-            float4 x[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const int i = i0 + u * GROUPS;
-                pm[u] = -INFINITY;
-                pl[u] = 0.f;
-                x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (i < n) {
-                    const int of = i < n0 ? first + i : i < n0 + n1 ? (cta0 + 1 + i - n0) * WARPS : cta1 * WARPS + i - n0 - n1;
-                    const float *from = part_of(p, warps, D, of, i == 0 ? 1 : 0);
-                    pm[u] = from[row];
-                    pl[u] = from[ROWS + row];
-                    x[u] = *reinterpret_cast<const float4 *>(from + 2 * ROWS + row * D + quad * 4);
-                }
-            }
-            const float m_new = fmaxf(m, fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3])));
-            const float mu = m_new == -INFINITY ? 0.f : m_new, keep = ex2(m - mu);
-            l *= keep;
-            acc.x *= keep; acc.y *= keep; acc.z *= keep; acc.w *= keep;
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const float f = ex2(pm[u] - mu);
-                l = fmaf(pl[u], f, l);
-                acc.x = fmaf(x[u].x, f, acc.x); acc.y = fmaf(x[u].y, f, acc.y);
-                acc.z = fmaf(x[u].z, f, acc.z); acc.w = fmaf(x[u].w, f, acc.w);
-            }
-            m = m_new;
-        }
+        if (!there(head)) continue;
+        const Parts parts(head, blockIdx.x * WARPS + w);
+        if (parts.n <= JOIN_FEW) continue;
+        Joined sum;
+        sum.add_parts<4>(p, warps, D, parts, row, quad, grp, GROUPS);
         if (quad == 0) {
-            m_s[grp] = m;
-            l_s[grp] = l;
+            m_s[grp] = sum.m;
+            l_s[grp] = sum.l;
         }
-        acc_s[grp][quad] = acc;
+        acc_s[grp][quad] = sum.acc;
         __syncthreads();
-        if (grp == 0) {
+        if (grp == 0) {                 // the groups' sums in order
+            float m = sum.m;
 #pragma unroll
-            for (int g = 0; g < GROUPS; ++g) m = fmaxf(m, m_s[g]);
-            const float mu = m == -INFINITY ? 0.f : m;
-            l = 0.f;
-            acc = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int g = 1; g < GROUPS; ++g) m = fmaxf(m, m_s[g]);
+            sum.rescale(m);
 #pragma unroll
-            for (int g = 0; g < GROUPS; ++g) {
-                const float4 x = acc_s[g][quad];
-                const float f = ex2(m_s[g] - mu);
-                l = fmaf(l_s[g], f, l);
-                acc.x = fmaf(x.x, f, acc.x); acc.y = fmaf(x.y, f, acc.y);
-                acc.z = fmaf(x.z, f, acc.z); acc.w = fmaf(x.w, f, acc.w);
-            }
-            const float inv = l == 0.f ? 0.f : 1.f / l;
-            const int h = head.hk * p.G + head.row0 + row;
-            T *out = reinterpret_cast<T *>(p.o) + (int64_t)head.b * p.o_sb + (int64_t)h * p.o_sh;
-            const float y[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (quad * 4 + e < p.d) out[quad * 4 + e] = from_f32<T>(y[e]);
-            if (p.lse && quad == 0) p.lse[(int64_t)head.b * p.Hq + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
+            for (int g = 1; g < GROUPS; ++g) sum.add(m_s[g], l_s[g], acc_s[g][quad]);
+            sum.store<T>(p, head, row, quad);
         }
-        __syncthreads();        // the next unit's parts go to the same shared memory
+        __syncthreads();                // the next unit's parts go to the same shared memory
     }
 }
 
