@@ -90,11 +90,42 @@ struct BwdParams {
     int across;                 // CTAs side by side
 };
 
-constexpr int BWD_WARPS = 4, BWD_THREADS = BWD_WARPS * 32;
+constexpr int BWD_WARPS = 4, BWD_THREADS = BWD_WARPS * 32, BWD_PER_SM = 6;
 constexpr int DIAGS = 32 * 8 + 7;       // of a warp's 32 neighbouring block diagonals
 
+// A row's eight elements and what lies around them up to 16-byte borders, and the elements out of that: `shift` of them
+// lie before the first.
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(BWD_THREADS) relbias_bwd_kernel(const __grid_constant__ BwdParams p) {
+struct Words {
+    static constexpr int PER = 16 / sizeof(T), N = 8 / PER + (VEC ? 0 : 1);
+    union {
+        uint4 u[N];
+        uint32_t w[N * 4];
+    };
+    __device__ __forceinline__ void read(const T *at, int shift) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) u[i] = ld_stream16(at - shift + i * PER);
+    }
+    __device__ __forceinline__ void elements(int shift, float (&x)[8]) {
+        if constexpr (!VEC) {
+            constexpr int WORD = 4 / sizeof(T);             // elements of a 32-bit word
+#pragma unroll
+            for (int s = 2; s >= 1; s /= 2)                 // by two words, by one
+#pragma unroll
+                for (int i = 0; i + s < N * 4; ++i) w[i] = shift & s * WORD ? w[i + s] : w[i];
+            if constexpr (sizeof(T) == 2)                   // by one element
+#pragma unroll
+                for (int i = 0; i + 1 < N * 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], shift & 1 ? 16 : 0);
+        }
+        const T *e = reinterpret_cast<const T *>(w);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) x[c] = to_f32<T>(e[c]);
+    }
+};
+
+// VEC: rows begin on 16 bytes.  Otherwise each row is read in the 16-byte words that its own alignment gives.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(BWD_THREADS, BWD_PER_SM) relbias_bwd_kernel(const __grid_constant__ BwdParams p) {
     __shared__ float diag[BWD_WARPS][DIAGS + 1];
     extern __shared__ float hist[];                     // [BWD_WARPS][buckets]
     __shared__ int at[MAX_SIDE];
@@ -111,65 +142,85 @@ __global__ void __launch_bounds__(BWD_THREADS) relbias_bwd_kernel(const __grid_c
 #pragma unroll
     for (int e = 0; e < 15; ++e) acc[e] = 0.f;
     const T *g = reinterpret_cast<const T *>(p.g) + (int64_t)h * p.g_sh;
+    const T *g_end = g + (int64_t)(p.Tq - 1) * p.g_sq + p.Tk;
     const int I1 = min(I0 + p.chunk, nI);
     for (int I = max(I0, -k); I < I1 && I + k < nJ; ++I) {
         const int i = I * 8, j = (I + k) * 8;
         const T *at0 = g + (int64_t)i * p.g_sq + j;
-        if (VEC && j + 8 <= p.Tk && i + 8 <= p.Tq) {
-            constexpr int PER = 16 / sizeof(T);
-            Vec<T, PER> x[8][8 / PER];
+        using W = Words<T, VEC>;
+        auto shift_of = [](const T *row) { return VEC ? 0 : (int)(reinterpret_cast<uintptr_t>(row) % 16 / sizeof(T)); };
+        const T *last = at0 + 7 * p.g_sq;
+        // the words of all eight rows lie between the matrix's first and last element
+        if (i + 8 <= p.Tq && at0 - shift_of(at0) >= g && last - shift_of(last) + W::N * W::PER <= g_end) {
+            constexpr int BATCH = 8 * sizeof(uint4) / sizeof(W);        // rows on their way at once: eight 16-byte words
 #pragma unroll
-            for (int r = 0; r < 8; ++r)
+            for (int r0 = 0; r0 < 8; r0 += BATCH) {
+                W words[BATCH];
 #pragma unroll
-                for (int c = 0; c < 8 / PER; ++c) x[r][c] = load_vec_stream<T, PER>(at0 + r * p.g_sq + c * PER);
+                for (int r = 0; r < BATCH; ++r) words[r].read(at0 + (r0 + r) * p.g_sq, shift_of(at0 + (r0 + r) * p.g_sq));
 #pragma unroll
-            for (int r = 0; r < 8; ++r)
+                for (int r = 0; r < BATCH; ++r) {
+                    float x[8];
+                    words[r].elements(shift_of(at0 + (r0 + r) * p.g_sq), x);
+                    if (j + 8 > p.Tk)
 #pragma unroll
-                for (int c = 0; c < 8; ++c) acc[c - r + 7] += to_f32<T>(x[r][c / PER].v[c % PER]);
+                        for (int c = 0; c < 8; ++c)
+                            if (j + c >= p.Tk) x[c] = 0.f;
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) acc[c - (r0 + r) + 7] += x[c];
+                }
+            }
         } else {
+            // at the matrix's ends: no branch between the reads, which would make each wait for the one before it
 #pragma unroll
-            for (int r = 0; r < 8; ++r)
+            for (int r0 = 0; r0 < 8; r0 += 4) {
+                T x[4][8];
 #pragma unroll
-                for (int c = 0; c < 8; ++c)
-                    if (i + r < p.Tq && j + c < p.Tk) acc[c - r + 7] += to_f32<T>(at0[r * p.g_sq + c]);
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int c = 0; c < 8; ++c)
+                        x[r][c] = i + r0 + r < p.Tq && j + c < p.Tk ? at0[(r0 + r) * p.g_sq + c] : from_f32<T>(0.f);
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) acc[c - (r0 + r) + 7] += to_f32<T>(x[r][c]);
+            }
         }
     }
     __syncthreads();
     // the warp's diagonals: j - i = 8 k_warp - 7 + index; neighbouring threads share seven of them
-#pragma unroll
-    for (int e = 0; e < 8; ++e) diag[warp][lane * 8 + e] = acc[e];
-    if (lane == 31)
-#pragma unroll
-        for (int e = 8; e < 15; ++e) diag[warp][lane * 8 + e] = acc[e];
-    __syncwarp();
-    if (lane < 31)
-#pragma unroll
-        for (int e = 8; e < 15; ++e) diag[warp][lane * 8 + e] += acc[e];
-    __syncwarp();
     const int lo = 8 * k_warp - 7 - p.offset, hi = lo + DIAGS - 1;
     float *mine = hist + warp * buckets;
     const int from = bucket_of(at, side, both, lo), to = bucket_of(at, side, both, hi);
-    for (int b = 0; b < buckets; ++b) {
-        // bucket b holds the differences [d0, d1]
-        if (from == to && b != from) continue;          // the whole window is in one bucket
-        const int s = b < side ? b : b - side;
-        const int near = s == 0 ? 0 : at[s - 1], far = s == side - 1 ? 1 << 30 : at[s] - 1;
-        int d0, d1;
-        if (b < side) {
-            d0 = -far;
-            d1 = s == 0 && !both ? 1 << 30 : -near;
-        } else {
-            d0 = max(near, 1);
-            d1 = far;
-        }
-        d0 = max(d0, lo);
-        d1 = min(d1, hi);
-        if (d0 > d1) continue;
+    if (from == to) {                   // all in one bucket
         float sum = 0.f;
-        for (int d = d0 + lane; d <= d1; d += 32) sum += diag[warp][d - lo];
+#pragma unroll
+        for (int e = 0; e < 15; ++e) sum += acc[e];
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (lane == 0) mine[b] = sum;
+        if (lane == 0) mine[from] = sum;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) diag[warp][lane * 8 + e] = acc[e];
+        if (lane == 31)
+#pragma unroll
+            for (int e = 8; e < 15; ++e) diag[warp][lane * 8 + e] = acc[e];
+        __syncwarp();
+        if (lane < 31)
+#pragma unroll
+            for (int e = 8; e < 15; ++e) diag[warp][lane * 8 + e] += acc[e];
+        __syncwarp();
+        // a lane per bucket, which holds the differences [d0, d1]
+        for (int b = lane; b < buckets; b += 32) {
+            const int s = b < side ? b : b - side;
+            const int near = s == 0 ? 0 : at[s - 1], far = s == side - 1 ? 1 << 30 : at[s] - 1;
+            const int d0 = max(b < side ? -far : max(near, 1), lo);
+            const int d1 = min(b >= side ? far : s == 0 && !both ? 1 << 30 : -near, hi);
+            float sum = 0.f;
+#pragma unroll 8
+            for (int d = d0; d <= d1; ++d) sum += diag[warp][d - lo];
+            mine[b] = sum;
+        }
     }
     __syncthreads();
     float *out = p.parts + ((int64_t)h * gridDim.x + blockIdx.x) * buckets;
@@ -201,7 +252,10 @@ BwdGrid bwd_grid(int64_t H, int64_t Tq, int64_t Tk) {
     int chunk = 32;
     auto across = [&] { return ceil_div64(nJ + chunk - 1, BWD_THREADS); };
     auto ctas = [&] { return ceil_div64(nI, chunk) * across(); };
-    while (chunk > 4 && H * ctas() < 8 * num_sms()) chunk /= 2;
+    for (; chunk > 4; chunk /= 2) {         // as few as still leave one wave
+        const int64_t half = ceil_div64(nI, chunk / 2) * ceil_div64(nJ + chunk / 2 - 1, BWD_THREADS);
+        if (H * half > BWD_PER_SM * num_sms()) break;
+    }
     return {chunk, (int)across(), (int)ctas()};
 }
 
