@@ -40,8 +40,8 @@ constexpr int APPEND_BATCH = 4;             // tokens that a thread reads before
 constexpr int APPEND_LOOP = 8;              // most tokens of a thread
 constexpr int ANGLE_BYTES = 16 << 10;       // shared memory for the angles of a CTA's tokens
 
-// Eight angles of a table row from element `at` on, `left` of them in the table, `past` in place of the others.
-__device__ __forceinline__ void load_angles(const AppendParams &p, int64_t at, int left, float past, float (&w)[8]) {
+// Eight angles of a table row from element `at` on, `left` of them in the table and zeros.
+__device__ __forceinline__ void load_angles(const AppendParams &p, int64_t at, int left, float (&w)[8]) {
     if (p.pos_vec && left >= 8) {
         if (p.pos_dtype == RGD_F32) {
             const float4 *f = reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(p.pos) + at);
@@ -60,7 +60,7 @@ __device__ __forceinline__ void load_angles(const AppendParams &p, int64_t at, i
         return;
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) w[e] = e < left ? load_as_f32(p.pos, at + e, p.pos_dtype) : past;
+    for (int e = 0; e < 8; ++e) w[e] = e < left ? load_as_f32(p.pos, at + e, p.pos_dtype) : 0.f;
 }
 
 // Where a token goes.
@@ -72,21 +72,22 @@ struct alignas(16) Place {
 // Each CTA has one of the three tensors and a few tokens of it, each thread one group of VE channels (16 bytes, or a
 // pair where views are not addressable that way) of one head after another.  Where the tokens go and their angles are
 // looked up once for the CTA, two dependent reads (length; table entry and angles) during which the first tokens are on
-// their way; the loop is then read, turn, write.  [4, 4096, 16, 128] bf16 keys, values and queries (411 MB): 78 us, 81 %
+// their way; the loop is then read, turn, write.  [4, 4096, 16, 128] bf16 keys, values and queries (411 MB): 76 us, 83 %
 // of the copy rate, bound by instruction issue (two thirds of the slots busy) and the look-ups.  With every thread
-// looking up its own tokens it executed 222 instructions per 16 bytes instead of 130 and took 160-200 us.
+// looking up its own tokens it executed 222 instructions per 16 bytes instead of 130 and took 160-200 us.  Four CTAs an
+// SM: at five the registers spill (84 us).
 template <typename T, int VE>
-__global__ void __launch_bounds__(APPEND_THREADS, 5) append_kernel(const __grid_constant__ AppendParams p) {
+__global__ void __launch_bounds__(APPEND_THREADS, 4) append_kernel(const __grid_constant__ AppendParams p) {
     using V = Vec<T, VE>;
     extern __shared__ __align__(16) unsigned char raw[];
     const int which = blockIdx.y, tid = threadIdx.x;
     const AppendGeo &g = p.geo[which == 2];
     const int heads = which == 2 ? p.Hq : p.Hkv, all = p.B * p.N, mine = g.loop * g.tokens;
+    if (heads == 0 || (int64_t)blockIdx.x * mine >= all) return;       // the grid is the larger one of two
     const int first = blockIdx.x * mine;
-    if (first >= all || heads == 0) return;
     Place *places = reinterpret_cast<Place *>(raw);             // [loop][tokens]
     // [loop][tokens], sines and cosines, first and second halves of the groups of 8 channels (a warp then reads 16 bytes
-    // next to 16 bytes); channels past R have sine 0 and cosine 1
+    // next to 16 bytes)
     float *angles = reinterpret_cast<float *>(places + mine);
     const int sub = (int)fdiv((uint32_t)tid, g.by_per_token), rest = tid - sub * g.per_token;
     const int row0 = (int)fdiv((uint32_t)rest, p.by_vecs), c = (rest - row0 * p.vecs) * VE;
@@ -154,7 +155,7 @@ __global__ void __launch_bounds__(APPEND_THREADS, 5) append_kernel(const __grid_
             const int position = first + t < all ? position_of(t) : -1;
             if (position < 0) continue;
             float w[8];
-            load_angles(p, position * p.pos_sn + cosine * p.pos_ss + q * 8, p.R - q * 8, cosine ? 1.f : 0.f, w);
+            load_angles(p, position * p.pos_sn + cosine * p.pos_ss + q * 8, p.R - q * 8, w);
             float *to = angles + (t * 2 + cosine) * 8 * groups + q * 4;
             *reinterpret_cast<float4 *>(to) = make_float4(w[0], w[1], w[2], w[3]);
             *reinterpret_cast<float4 *>(to + 4 * groups) = make_float4(w[4], w[5], w[6], w[7]);
@@ -164,6 +165,7 @@ __global__ void __launch_bounds__(APPEND_THREADS, 5) append_kernel(const __grid_
     if (!works) return;
 
     const bool turns = turned && c < p.R;
+    const int rotated = p.R - c;                            // channels of the group, and more where all are
     const int quarter = 4 * p.angle_groups;                 // floats of one half of the groups
     const float *sin0 = angles + sub * 4 * quarter + (c / 8) * 4 + (VE == 8 ? 0 : (c / 4) % 2 * quarter + c % 4);
     for (int row = row0; row < heads; row += g.step) {
@@ -184,6 +186,7 @@ __global__ void __launch_bounds__(APPEND_THREADS, 5) append_kernel(const __grid_
                         const W sw = *reinterpret_cast<const W *>(sin + e / 4 * quarter), cw = *reinterpret_cast<const W *>(cos + e / 4 * quarter);
 #pragma unroll
                         for (int k = 0; k < (VE == 8 ? 4 : 2); k += 2) {
+                            if (e + k >= rotated) break;            // R is even: a rotated pair is whole
                             const float x0 = to_f32<T>(v[u].v[e + k]), x1 = to_f32<T>(v[u].v[e + k + 1]);
                             *reinterpret_cast<uint32_t *>(&v[u].v[e + k]) =
                                 attn::Mma<T>::pack(x0 * cw.v[k] - x1 * sw.v[k], x1 * cw.v[k + 1] + x0 * sw.v[k + 1]);
@@ -279,7 +282,7 @@ extern "C" int rgd_paged_append(const rgd_heads *key, const rgd_heads *value, co
     if (dtype != RGD_F16 && dtype != RGD_BF16) return RGD_E_DTYPE;
     if (pos && !dtype_ok(pos_dtype)) return RGD_E_DTYPE;
     if (B < 0 || N < 0 || Hq < 0 || Hkv < 0 || d < 0) return RGD_E_INVALID;
-    if (d > 128 || Hq > 65535 || Hkv > 65535 || B > INT32_MAX || N > INT32_MAX || B * N > INT32_MAX) return RGD_E_SIZE;
+    if (d > 128 || Hq > 65535 || Hkv > 65535 || B > 1 << 30 || N > 1 << 30 || B * N > 1 << 30) return RGD_E_SIZE;
     if (pos && (P < 0 || R < 0 || R > d || R % 2 != 0)) return RGD_E_INVALID;
     if (int e = paged::check_paged(cache, B, Hkv > 0 && d > 0)) return e;
     if (!query) Hq = 0;

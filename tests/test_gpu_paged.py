@@ -106,6 +106,44 @@ def test_append_around_the_cache_changes_nothing():
     assert torch.equal(mine.cpu(), want)
 
 
+@pytest.mark.parametrize("R", [6, 12, 20, 34])
+def test_channels_past_the_rotated_ones_are_copied_bit_for_bit(R):
+    """Infinities, NaN and negative zeros there, next to rotated channels in one 16-byte group."""
+    g = gen(R)
+    d, page = 64, 16
+    key = randn(g, 2, 7, 3, d, dtype=torch.float16)
+    special = torch.tensor([math.inf, -math.inf, math.nan, -0.0, 0.0, -2.5], dtype=torch.float16)
+    key[..., R:] = special[torch.randint(0, 6, key[..., R:].shape, generator=g)]
+    table, lengths = torch.tensor([[1, 0], [3, 2]], dtype=torch.int32), torch.tensor([3, 12], dtype=torch.int32)
+    kc, vc = (torch.zeros(4, page, 3, d, dtype=torch.float16) for _ in range(2))
+    k_gpu, v_gpu = kc.cuda(), vc.cuda()
+    q = F_.paged_cache_append_fn(key.cuda(), key.cuda(), k_gpu, v_gpu, table.cuda(), lengths.cuda(), rotary_table(64, R, torch.float32).cuda(), key.cuda())
+    bits = lambda t: t.cpu().contiguous().view(torch.int16)
+    assert torch.equal(bits(q[..., R:]), bits(key[..., R:]))
+    for b in range(2):
+        for i in range(7):
+            at = P.locate(table, b, int(lengths[b]) + i, page, 4)
+            assert torch.equal(bits(k_gpu[at][..., R:]), bits(key[b, i][..., R:])) and torch.equal(bits(v_gpu[at]), bits(key[b, i]))
+            assert torch.isfinite(k_gpu[at][..., :R]).all()
+
+
+def test_append_of_many_tokens_with_few_and_many_heads():
+    """Grids of the caches and of the query that differ by more than a hundred times, and tokens that cross sequences."""
+    g = gen(77)
+    B, N, Hq, Hk, d = 3, 1500, 96, 1, 8
+    lengths = torch.tensor([0, 7, 100], dtype=torch.int32)
+    table, pages = _table(g, [int(n) + N for n in lengths], 32)
+    kc, vc = _pool(g, pages, 32, Hk, d, torch.bfloat16)
+    key, value, query = (randn(g, B, N, h, d, dtype=torch.bfloat16) for h in (Hk, Hk, Hq))
+    pos = rotary_table(1700, d, torch.bfloat16)
+    k_gpu, v_gpu = kc.cuda(), vc.cuda()
+    q = F_.paged_cache_append_fn(key.cuda(), value.cuda(), k_gpu, v_gpu, table.cuda(), lengths.cuda(), pos.cuda(), query.cuda())
+    (wk, wv, wq), (sk, _, sq) = P.append(key, value, kc, vc, table, lengths, pos, query)
+    P.assert_rotated(k_gpu.cpu(), wk, sk, "k_cache")
+    assert torch.equal(v_gpu.cpu().double(), wv)
+    P.assert_rotated(q.cpu(), wq, sq, "query")
+
+
 def test_append_leaves_out_what_has_no_place():
     """Bad pages, positions past the table or the rotary table, negative lengths: not written, and reported."""
     g = gen(2)
