@@ -28,6 +28,8 @@ struct AttnParams {
     float *lse;                             // null: not wanted
     int B, Hq, Hkv, G, d;                   // G: query heads of a cache head
     int groups, units;                      // row tiles of a cache head, of a sequence
+    FastDiv by_units, by_groups;
+    int direct;                             // a CTA per unit, nothing to join
     char *work;
     float scale_log2;
     const void *w;                          // null: no position bias
@@ -115,7 +117,8 @@ __device__ __forceinline__ float *part_of(const AttnParams &p, int warps, int D,
 
 // The costs [0, total) dealt out to the warps: equal shares, the first ones with one more.
 struct Runs {
-    int total, busy, share, more;       // busy: warps with a share
+    int total = 0, busy = 0, share = 0, more = 0;       // busy: warps with a share
+    Runs() = default;
     __device__ __forceinline__ Runs(int total, int warps) : total(total) {
         busy = total == 0 ? 0 : max(1, min(warps, total / MIN_COST));       // a share is at least MIN_COST: a tile
         share = busy > 0 ? (int)((unsigned)total / (unsigned)busy) : 0;
@@ -146,78 +149,96 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attn_kernel(const __grid
     auto tiles_of = [](int len) { return (len + KEYS - 1) / KEYS; };
     auto cost_of = [&](int tiles) { return tiles > 0 ? tiles + UNIT_COST : 0; };
 
-    // cost of a head's units before each sequence: every thread sums a run of sequences, then the runs are added up
-    const int chunk = (p.B + THREADS - 1) / THREADS, b0 = min(tid * chunk, p.B), b1 = min(b0 + chunk, p.B);
-    int mine = 0, filled = 0;                               // cost; sequences with a token
-    for (int b = b0; b < b1; ++b) {
-        const int tiles = tiles_of(live_length(p, b, blockIdx.x == 0));
-        mine += cost_of(tiles);
-        filled += tiles > 0;
-    }
-    int upto = mine, filled_upto = filled;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int x = __shfl_up_sync(0xffffffffu, upto, o), y = __shfl_up_sync(0xffffffffu, filled_upto, o);
-        if (lane >= o) {
-            upto += x;
-            filled_upto += y;
-        }
-    }
-    if (lane == 31) {
-        sm.sums[warp] = upto;
-        sm.counts[warp] = filled_upto;
-    }
-    if (BIAS)
+    if (BIAS) {
         for (int k = tid; k < p.borders.side - 1; k += THREADS) sm.borders[k] = p.borders.at[k];
-    __syncthreads();
-    int all = 0;
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
-        if (w < warp) {
-            upto += sm.sums[w];
-            filled_upto += sm.counts[w];
-        }
-        all += sm.sums[w];
+        if (p.direct) __syncthreads();
     }
-    const Runs runs(all * p.units, warps);
-    // the boundaries of this CTA's runs: the thread whose sequences a boundary lies in finds it.  A unit's cost comes
-    // before its tiles.
-#pragma unroll
-    for (int w = 0; w <= WARPS; ++w) {
-        const int pos = runs.begin((int)blockIdx.x * WARPS + w);
-        int before = upto - mine, filled_before = filled_upto - filled;
-        if (pos >= before * p.units && pos < upto * p.units) {
-            for (int b = b0; b < b1; ++b) {
-                const int tiles = tiles_of(live_length(p, b, false)), cost = cost_of(tiles);
-                if (pos < (before + cost) * p.units) {
-                    const int in = pos - before * p.units, unit = (int)((unsigned)in / (unsigned)cost), tile = max(in - unit * cost - UNIT_COST, 0);
-                    sm.at[w] = {(before - filled_before * UNIT_COST) * p.units + unit * tiles + tile, b, unit, tile};
-                    break;
-                }
-                before += cost;
-                filled_before += tiles > 0;
-            }
-        } else if (tid == THREADS - 1 && pos >= runs.total) {
-            sm.at[w] = {(all - filled_upto * UNIT_COST) * p.units, p.B, 0, 0};
-        }
-    }
-    __syncthreads();
-    const int n = sm.at[warp + 1].tiles - sm.at[warp].tiles;
-    if (lane == 0) reinterpret_cast<Header *>(p.work)[me].last = -1;
-    const bool merge = sm.at[0].b < p.B && sm.at[0].b == sm.at[WARPS].b && sm.at[0].unit == sm.at[WARPS].unit;
-
     Cursor at{}, to{};          // of the tile that is computed, of the tile whose table entries are fetched next
-    if (n > 0) {
-        at.b = sm.at[warp].b;
-        at.len = live_length(p, at.b, false);
+    Runs runs{};
+    int n;
+    bool merge;                 // the warps' parts are added up in the CTA
+    if (p.direct) {
+        // one CTA's unit; its warps take every fourth tile
+        at.b = (int)fdiv(blockIdx.x, p.by_units);
+        const int unit = (int)blockIdx.x - at.b * p.units;
+        at.len = live_length(p, at.b, unit == 0);
         at.tiles = tiles_of(at.len);
-        at.tile = sm.at[warp].tile;
-        at.hk = (int)((unsigned)sm.at[warp].unit / (unsigned)p.groups);
-        at.group = sm.at[warp].unit - at.hk * p.groups;
-        to = at;
+        at.hk = (int)fdiv((uint32_t)unit, p.by_groups);
+        at.group = unit - at.hk * p.groups;
+        at.tile = warp;
+        n = at.tiles > warp ? (at.tiles - warp + WARPS - 1) / WARPS : 0;
+        merge = true;
+    } else {
+        // cost of a head's units before each sequence: every thread sums a run of sequences, then the runs are added up
+        const int chunk = (p.B + THREADS - 1) / THREADS, b0 = min(tid * chunk, p.B), b1 = min(b0 + chunk, p.B);
+        int mine = 0, filled = 0;                               // cost; sequences with a token
+        for (int b = b0; b < b1; ++b) {
+            const int tiles = tiles_of(live_length(p, b, blockIdx.x == 0));
+            mine += cost_of(tiles);
+            filled += tiles > 0;
+        }
+        int upto = mine, filled_upto = filled;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, upto, o), y = __shfl_up_sync(0xffffffffu, filled_upto, o);
+            if (lane >= o) {
+                upto += x;
+                filled_upto += y;
+            }
+        }
+        if (lane == 31) {
+            sm.sums[warp] = upto;
+            sm.counts[warp] = filled_upto;
+        }
+        __syncthreads();
+        int all = 0;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+            if (w < warp) {
+                upto += sm.sums[w];
+                filled_upto += sm.counts[w];
+            }
+            all += sm.sums[w];
+        }
+        runs = Runs(all * p.units, warps);
+        // the boundaries of this CTA's runs: the thread whose sequences a boundary lies in finds it.  A unit's cost comes
+        // before its tiles.
+#pragma unroll
+        for (int w = 0; w <= WARPS; ++w) {
+            const int pos = runs.begin((int)blockIdx.x * WARPS + w);
+            int before = upto - mine, filled_before = filled_upto - filled;
+            if (pos >= before * p.units && pos < upto * p.units) {
+                for (int b = b0; b < b1; ++b) {
+                    const int tiles = tiles_of(live_length(p, b, false)), cost = cost_of(tiles);
+                    if (pos < (before + cost) * p.units) {
+                        const int in = pos - before * p.units, unit = (int)((unsigned)in / (unsigned)cost), tile = max(in - unit * cost - UNIT_COST, 0);
+                        sm.at[w] = {(before - filled_before * UNIT_COST) * p.units + unit * tiles + tile, b, unit, tile};
+                        break;
+                    }
+                    before += cost;
+                    filled_before += tiles > 0;
+                }
+            } else if (tid == THREADS - 1 && pos >= runs.total) {
+                sm.at[w] = {(all - filled_upto * UNIT_COST) * p.units, p.B, 0, 0};
+            }
+        }
+        __syncthreads();
+        n = sm.at[warp + 1].tiles - sm.at[warp].tiles;
+        if (lane == 0) reinterpret_cast<Header *>(p.work)[me].last = -1;
+        merge = sm.at[0].b < p.B && sm.at[0].b == sm.at[WARPS].b && sm.at[0].unit == sm.at[WARPS].unit;
+        if (n > 0) {
+            at.b = sm.at[warp].b;
+            at.len = live_length(p, at.b, false);
+            at.tiles = tiles_of(at.len);
+            at.tile = sm.at[warp].tile;
+            at.hk = (int)fdiv((uint32_t)sm.at[warp].unit, p.by_groups);
+            at.group = sm.at[warp].unit - at.hk * p.groups;
+        }
     }
+    to = at;
     auto advance = [&](Cursor &c) {
-        if (++c.tile < c.tiles) return;
+        c.tile += p.direct ? WARPS : 1;
+        if (p.direct || c.tile < c.tiles) return;
         c.tile = 0;
         if (++c.group < p.groups) return;
         c.group = 0;
@@ -282,7 +303,11 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attn_kernel(const __grid
     };
     uint32_t aq[D / 16][4];             // the unit's queries as A fragments, rows past the group and channels past d as zeros
     float o[NT][4];                     // rows gq and gq + 8
-    float m_ref[2], l_sum[2];
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[j][e] = 0.f;          // a warp without a tile has its part in a unit's end too
+    float m_ref[2] = {-INFINITY, -INFINITY}, l_sum[2] = {0.f, 0.f};
     bool whole = false;                 // the unit's first tile was in this run
     const int mi = lane >> 3, mr = lane & 7;
 
@@ -440,7 +465,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attn_kernel(const __grid
         for (int j = 0; j < STAGES; ++j) live[j] = live[j + 1];
 
         const bool done = at.tile == at.tiles - 1;
-        if (done || i == n - 1) {
+        if (!p.direct && (done || i == n - 1)) {
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
                 l_sum[r] += __shfl_xor_sync(0xffffffffu, l_sum[r], 1);
@@ -488,14 +513,23 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attn_kernel(const __grid
     asm volatile("cp.async.wait_group 0;" ::: "memory");
 
     if (merge) {                // uniform over the CTA; the rings are done with
-        const typename S::Boundary begins = sm.at[0];
-        const int hk = begins.unit / p.groups, rows = min(ROWS, p.G - (begins.unit - hk * p.groups) * ROWS);
+        // the CTA's unit, which a warp without a tile knows from the schedule alone
+        int hk = at.hk, group = at.group;
+        if (!p.direct) {
+            hk = (int)fdiv((uint32_t)sm.at[0].unit, p.by_groups);
+            group = sm.at[0].unit - hk * p.groups;
+        }
+        const int rows = min(ROWS, p.G - group * ROWS), h0 = hk * p.G + group * ROWS;
         float *mine_o = reinterpret_cast<float *>(sm.ring[warp]), *mine_m = mine_o + ROWS * D;       // then the sums
         static_assert(sizeof(sm.ring[0]) >= part_floats(D) * sizeof(float), "a part in a warp's ring");
         __syncwarp();
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
             const int row = gq + r * 8;
+            if (p.direct) {             // a run's end has done it otherwise
+                l_sum[r] += __shfl_xor_sync(0xffffffffu, l_sum[r], 1);
+                l_sum[r] += __shfl_xor_sync(0xffffffffu, l_sum[r], 2);
+            }
             if (tq == 0) {
                 mine_m[row] = m_ref[r];
                 mine_m[ROWS + row] = l_sum[r];
@@ -504,7 +538,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attn_kernel(const __grid
             for (int j = 0; j < NT; ++j) *reinterpret_cast<float2 *>(mine_o + row * D + j * 8 + tq * 2) = make_float2(o[j][2 * r], o[j][2 * r + 1]);
         }
         __syncthreads();
-        float *part = part_of(p, warps, D, blockIdx.x * WARPS, begins.tile == 0 ? 1 : 0);
+        float *part = p.direct ? nullptr : part_of(p, warps, D, blockIdx.x * WARPS, sm.at[0].tile == 0 ? 1 : 0);
         for (int e = tid; e < rows * (D / 4); e += THREADS) {
             const int row = e / (D / 4), c = e % (D / 4) * 4;
             const float *from[WARPS];
@@ -524,16 +558,25 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attn_kernel(const __grid
                 y.x = fmaf(x.x, f, y.x); y.y = fmaf(x.y, f, y.y);
                 y.z = fmaf(x.z, f, y.z); y.w = fmaf(x.w, f, y.w);
             }
-            *reinterpret_cast<float4 *>(part + 2 * ROWS + row * D + c) = y;
-            if (c == 0) {
-                part[row] = m;
-                part[ROWS + row] = l;
+            if (!p.direct) {
+                *reinterpret_cast<float4 *>(part + 2 * ROWS + row * D + c) = y;
+                if (c == 0) {
+                    part[row] = m;
+                    part[ROWS + row] = l;
+                }
+                continue;
             }
+            const float inv = l == 0.f ? 0.f : 1.f / l, z[4] = {y.x * inv, y.y * inv, y.z * inv, y.w * inv};
+            T *out = reinterpret_cast<T *>(p.o) + (int64_t)at.b * p.o_sb + (int64_t)(h0 + row) * p.o_sh + c;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (c + k < p.d) out[k] = from_f32<T>(z[k]);
+            if (c == 0 && p.lse) p.lse[(int64_t)at.b * p.Hq + h0 + row] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
         }
     }
 
     // sequences without a token
-    for (int b = blockIdx.x; b < p.B; b += gridDim.x)
+    for (int b = blockIdx.x; !p.direct && b < p.B; b += gridDim.x)
         if (live_length(p, b, false) == 0) {
             T *out = reinterpret_cast<T *>(p.o) + (int64_t)b * p.o_sb;
             for (int e = tid; e < p.Hq * p.d; e += THREADS) {
@@ -670,30 +713,36 @@ bool too_large(int64_t B, int64_t units, int64_t max_keys, int D) {
     return (double)B * (double)units * (double)(ceil_div64(max_keys, tile_keys(D)) + UNIT_COST) > (double)INT32_MAX;
 }
 
-// CTAs of the grid: what the SMs hold at once, and no more than there can be runs.
-int grid_size(int64_t B, int64_t units, int64_t max_keys, int D, int resident) {
-    const int64_t most = B * units * (ceil_div64(max_keys, tile_keys(D)) + UNIT_COST);
-    const int64_t room = (int64_t)num_sms() * resident;
-    const int64_t n = ceil_div64(most, MIN_COST * WARPS);
-    return (int)(n < 1 ? 1 : n < room ? n : room);
+// How the tiles are spread.  Tables for few keys: a CTA per unit, which needs no schedule, no workspace and no second
+// launch.  Others: what the SMs hold at once, and no more CTAs than there can be runs.
+constexpr int DIRECT_TILES = 32;
+struct Plan {
+    bool direct;
+    int grid;
+};
+Plan make_plan(int64_t B, int64_t units, int64_t max_keys, int D) {
+    const int64_t tiles = ceil_div64(max_keys, tile_keys(D));
+    if (tiles <= DIRECT_TILES) return {true, (int)(B * units)};
+    const int64_t n = ceil_div64(B * units * (tiles + UNIT_COST), MIN_COST * WARPS), room = (int64_t)num_sms() * CTAS_PER_SM;
+    return {false, (int)(n < room ? n : room)};
 }
 
 template <typename T, int D, bool VEC, bool BIAS>
-int launch(AttnParams &p, int64_t max_keys, cudaStream_t st) {
+int launch(AttnParams &p, const Plan &plan, cudaStream_t st) {
     auto kernel = attn_kernel<T, D, VEC, BIAS>;
     constexpr size_t smem = sizeof(Smem<T, D>);
     static_assert(CTAS_PER_SM * (smem + 1024) <= 228 << 10, "shared memory of an SM");
     if (int e = ensure_dyn_smem(reinterpret_cast<const void *>(kernel), smem)) return e;
-    const int grid = grid_size(p.B, p.units, max_keys, D, CTAS_PER_SM);
-    kernel<<<grid, THREADS, smem, st>>>(p);
+    kernel<<<plan.grid, THREADS, smem, st>>>(p);
     count_launch();
     if (int e = check_launch()) return e;
-    return sm100::launch_pdl(join_kernel<T, D>, dim3(grid, (unsigned)(p.G < ROWS ? p.G : ROWS)), JOIN_THREADS, 0, st, p);
+    if (plan.direct) return RGD_OK;
+    return sm100::launch_pdl(join_kernel<T, D>, dim3(plan.grid, (unsigned)(p.G < ROWS ? p.G : ROWS)), JOIN_THREADS, 0, st, p);
 }
 template <typename T, int D>
-int launch(AttnParams &p, bool vec, int64_t max_keys, cudaStream_t st) {
-    if (p.w) return vec ? launch<T, D, true, true>(p, max_keys, st) : launch<T, D, false, true>(p, max_keys, st);
-    return vec ? launch<T, D, true, false>(p, max_keys, st) : launch<T, D, false, false>(p, max_keys, st);
+int launch(AttnParams &p, bool vec, const Plan &plan, cudaStream_t st) {
+    if (p.w) return vec ? launch<T, D, true, true>(p, plan, st) : launch<T, D, false, true>(p, plan, st);
+    return vec ? launch<T, D, true, false>(p, plan, st) : launch<T, D, false, false>(p, plan, st);
 }
 
 int status_fetch() {
@@ -722,7 +771,8 @@ extern "C" int64_t rgd_paged_attn_workspace_bytes(int64_t B, int64_t Hq, int64_t
     const int D = d > 64 ? 128 : 64;
     const int64_t units = Hkv * ceil_div64(Hq / Hkv, paged::ROWS);
     if (paged::too_large(B, units, max_pages * page_size, D)) return RGD_E_SIZE;
-    return paged::workspace_bytes(paged::grid_size(B, units, max_pages * page_size, D, paged::CTAS_PER_SM), D);
+    const paged::Plan plan = paged::make_plan(B, units, max_pages * page_size, D);
+    return plan.direct ? 0 : paged::workspace_bytes(plan.grid, D);
 }
 
 extern "C" int rgd_paged_attn(const rgd_heads *q, const rgd_paged *cache, const rgd_relbias *bias, const rgd_heads *o, float *lse,
@@ -754,15 +804,18 @@ extern "C" int rgd_paged_attn(const rgd_heads *q, const rgd_paged *cache, const 
     }
     p.groups = (p.G + paged::ROWS - 1) / paged::ROWS;
     p.units = p.Hkv * p.groups;
+    p.by_units = make_fastdiv((uint32_t)p.units);
+    p.by_groups = make_fastdiv((uint32_t)p.groups);
     const int64_t max_keys = cache->max_pages * cache->page_size;
     const int64_t need = rgd_paged_attn_workspace_bytes(B, Hq, Hkv, d, cache->max_pages, cache->page_size);
     if (need < 0) return (int)need;
-    if (workspace_bytes < need || !workspace) return RGD_E_WORKSPACE;
-    if (!is_aligned(workspace, 16)) return RGD_E_STRIDE;
+    if (need > 0 && (workspace_bytes < need || !workspace)) return RGD_E_WORKSPACE;
+    if (need > 0 && !is_aligned(workspace, 16)) return RGD_E_STRIDE;
     p.work = reinterpret_cast<char *>(workspace);
     const bool vec = d % 8 == 0 && paged::cache_vec16(*cache) && paged::heads_vec16(*q) && paged::heads_vec16(*o);
     cudaStream_t st = (cudaStream_t)stream;
-    if (d > 64)
-        return dtype == RGD_BF16 ? paged::launch<__nv_bfloat16, 128>(p, vec, max_keys, st) : paged::launch<__half, 128>(p, vec, max_keys, st);
-    return dtype == RGD_BF16 ? paged::launch<__nv_bfloat16, 64>(p, vec, max_keys, st) : paged::launch<__half, 64>(p, vec, max_keys, st);
+    const paged::Plan plan = paged::make_plan(B, p.units, max_keys, d > 64 ? 128 : 64);
+    p.direct = plan.direct;
+    if (d > 64) return dtype == RGD_BF16 ? paged::launch<__nv_bfloat16, 128>(p, vec, plan, st) : paged::launch<__half, 128>(p, vec, plan, st);
+    return dtype == RGD_BF16 ? paged::launch<__nv_bfloat16, 64>(p, vec, plan, st) : paged::launch<__half, 64>(p, vec, plan, st);
 }
