@@ -713,18 +713,24 @@ bool too_large(int64_t B, int64_t units, int64_t max_keys, int D) {
     return (double)B * (double)units * (double)(ceil_div64(max_keys, tile_keys(D)) + UNIT_COST) > (double)INT32_MAX;
 }
 
-// How the tiles are spread.  Tables for few keys: a CTA per unit, which needs no schedule, no workspace and no second
-// launch.  Others: what the SMs hold at once, and no more CTAs than there can be runs.
-constexpr int DIRECT_TILES = 32;
+// How the tiles are spread.  Few units of few keys (by what the table has room for; the lengths are not known here): a CTA
+// per unit, which needs no schedule, no workspace and no second launch.  Others: what the SMs hold at once, and no more
+// CTAs than there can be runs.  us of GPU time in equal runs / a CTA per unit, at 8, 16, 24, 32, 48 tiles:
+//   16 units, head_dim 128    16.4 / 10.2   16.4 / 14.3   18.4 / 16.4   18.4 / 18.4   18.4 / 24.6
+//   256 units, head_dim 64    18.4 / 12.3   20.5 / 16.4   24.6 / 20.5   26.6 / 24.6   32.8 / 30.7
+//   512 units, head_dim 128   22.5 / 20.5   26.6 / 26.6   34.8 / 34.8   41.0 / 41.0   51.2 / 53.2
+//   2048 units, head_dim 128  41.0 / 53.2   63.5 / 75.8   84.0 / 102    107 / 125     147 / 168
+constexpr int DIRECT_TILES = 28;
 struct Plan {
     bool direct;
     int grid;
 };
 Plan make_plan(int64_t B, int64_t units, int64_t max_keys, int D) {
     const int64_t tiles = ceil_div64(max_keys, tile_keys(D));
-    if (tiles <= DIRECT_TILES) return {true, (int)(B * units)};
-    const int64_t n = ceil_div64(B * units * (tiles + UNIT_COST), MIN_COST * WARPS), room = (int64_t)num_sms() * CTAS_PER_SM;
-    return {false, (int)(n < room ? n : room)};
+    const int64_t room = (int64_t)num_sms() * CTAS_PER_SM;
+    if (tiles <= DIRECT_TILES && B * units <= room) return {true, (int)(B * units)};
+    const int64_t n = ceil_div64(B * units * (tiles + UNIT_COST), MIN_COST * WARPS);
+    return {false, (int)(n < 1 ? 1 : n < room ? n : room)};
 }
 
 template <typename T, int D, bool VEC, bool BIAS>
