@@ -439,7 +439,8 @@ int rgd_paged_slot(const rgd_paged *cache, int64_t row, int64_t position,
  * are copied.  fp32 arithmetic, one rounding.  A token whose position is not in
  * the cache or not below P is not written.  Two tokens of one call that map to
  * the same slot leave either's values there, channel by channel.  dtype RGD_F16
- * / RGD_BF16, pos_dtype any, d <= 128. */
+ * / RGD_BF16, pos_dtype any, d <= 128, B * N <= 2^30, max_pages * page_size below
+ * 2^31 - 1024. */
 int rgd_paged_append(const rgd_heads *key, const rgd_heads *value,
                      const rgd_heads *query, const rgd_heads *query_out,
                      const rgd_paged *cache, const int32_t *counts,
@@ -461,7 +462,8 @@ int64_t rgd_paged_attn_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv,
  * without a usable page.  Keys of pages out of range are left out.  dtype
  * RGD_F16 / RGD_BF16, d <= 128, Hq a multiple of Hkv, B * Hkv * ceil(Hq / Hkv /
  * 16) * (max_pages * page_size / 16 + 3) below 2^31.  The order of all sums
- * depends on the lengths and the device alone, not on the run. */
+ * depends on the lengths, max_pages, page_size and the device, not on the run:
+ * results are bit-reproducible. */
 int rgd_paged_attn(const rgd_heads *q, const rgd_paged *cache,
                    const rgd_relbias *bias, const rgd_heads *o, float *lse,
                    int64_t B, int64_t Hq, int64_t Hkv, int64_t d,

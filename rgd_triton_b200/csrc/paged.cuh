@@ -34,6 +34,8 @@ inline PagedView make_view(const rgd_paged &c) {
 inline int check_paged(const rgd_paged *c, int64_t B, bool cache_needed) {
     if (!c) return RGD_E_NULL;
     if (c->num_pages < 0 || c->max_pages < 0 || c->page_size < 1 || c->table_stride < 0) return RGD_E_INVALID;
+    if (c->k_stride_p < 0 || c->k_stride_s < 0 || c->k_stride_h < 0 || c->v_stride_p < 0 || c->v_stride_s < 0 || c->v_stride_h < 0)
+        return RGD_E_STRIDE;
     if (c->num_pages > INT32_MAX || c->page_size > INT32_MAX || c->max_pages > INT32_MAX ||
         c->max_pages * c->page_size > INT32_MAX - 1024)
         return RGD_E_SIZE;

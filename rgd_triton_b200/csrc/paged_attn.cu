@@ -57,7 +57,11 @@ __device__ __forceinline__ int live_length(const AttnParams &p, int b, bool repo
 // Two forms in which the four warps of a CTA shared a unit were slower: with the maxima and weights of a tile exchanged
 // and the channels split, three barriers a tile held the loop (120 us for one sequence of 131 thousand keys, 93 us like
 // this); with 16 keys of a tile each, added up at the unit's end, short sequences paid for that (103 us for 64 of 16
-// to 8192 keys).
+// to 8192 keys, 75 like this).
+//
+// One B200, cold L2: 64 sequences of 16 to 8192 keys, 32 / 8 heads of 128 (366 MB) 75 us, one of 131 thousand (537 MB)
+// 97-104 us.  Once the rings are full the keys arrive at 6.8 TB/s; 7 us go by before (lengths, table entries and first
+// tiles are reads that wait for one another), the warps end within 10 % of one another, and the join takes 3 us.
 //
 // Weights are split into two numbers of the cache's type (hi + lo): rounded to one, they would cost as much accuracy
 // as the output's own rounding, and the matrix pipe idles anyway.
@@ -256,11 +260,11 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attn_kernel(const __grid
     // all lanes copy the rows, 16 bytes each.
     const int my_key = lane % KEYS;
     struct Fetched {
-        int entry, slot, hk;        // entry -1: nothing to read
+        int entry, slot, hk;        // slot -1: past the sequence
     };
     uint32_t live[STAGES + 1] = {};             // which of the keys of tile i, i + 1, ... there are
     auto fetch = [&]() {
-        Fetched f{-1, 0, to.hk};
+        Fetched f{-1, -1, to.hk};
         const int key = to.tile * KEYS + my_key;
         if (key < to.len) {
             int index;
@@ -271,8 +275,8 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attn_kernel(const __grid
         return f;
     };
     auto find = [&](const Fetched &f, int i) {
-        const bool ok = page_ok(p.view, f.entry);
-        if (f.entry != -1 && !ok) g_attn_status = 1;
+        const bool ok = f.slot >= 0 && page_ok(p.view, f.entry);
+        if (f.slot >= 0 && !ok) g_attn_status = 1;
         if (KEYS == 32 || lane < KEYS) sm.row[warp][i & 1][lane] = ok ? f.entry * p.k_sp + f.slot * p.k_ss + f.hk * p.k_sh : -1;
         if (KEYS == 32 || lane >= KEYS)
             sm.row[warp][i & 1][KEYS + my_key] = ok ? f.entry * p.v_sp + f.slot * p.v_ss + f.hk * p.v_sh : -1;
@@ -331,7 +335,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attn_kernel(const __grid
     };
 
     static_assert(STAGES == 3, "the steps below are three tiles long");
-    Fetched next{-1, 0, 0};             // of tile i + STAGES once tile i is computed
+    Fetched next{-1, -1, 0};            // of tile i + STAGES once tile i is computed
     if (n > 0) {
         Fetched f[STAGES];              // the first tiles' entries together: one wait
 #pragma unroll
@@ -799,7 +803,8 @@ extern "C" int rgd_paged_attn(const rgd_heads *q, const rgd_paged *cache, const 
     p.lengths = cache->lengths;
     p.q = q->ptr; p.q_sb = q->stride_b; p.q_sh = q->stride_h;
     p.k = cache->k; p.k_sp = cache->k_stride_p; p.k_ss = cache->k_stride_s; p.k_sh = cache->k_stride_h;
-    p.v = cache->v; p.v_sp = cache->v_stride_p; p.v_ss = cache->v_stride_s; p.v_sh = cache->v_stride_h;
+    if (!p.k || !cache->v) p.k = q->ptr;            // no page: an address that no copy reads from
+    p.v = cache->v ? cache->v : p.k; p.v_sp = cache->v_stride_p; p.v_ss = cache->v_stride_s; p.v_sh = cache->v_stride_h;
     p.o = o->ptr; p.o_sb = o->stride_b; p.o_sh = o->stride_h;
     p.lse = lse;
     p.B = (int)B; p.Hq = (int)Hq; p.Hkv = (int)Hkv; p.G = (int)(Hq / Hkv); p.d = (int)d;

@@ -1313,7 +1313,7 @@ def _paged_attn_launch(q, k_cache, v_cache, page_table, lengths, softmax_scale, 
     _require(q.ndim == 4 and q.shape[1] == 1, f"q must be (batch, 1, nheads, headdim), got {tuple(q.shape)}")
     batch, _, nheads, d = q.shape
     _require(q.dtype in (torch.float16, torch.bfloat16), "Only support fp16 and bf16")
-    _require(d <= 128, "FlashAttention only support head dimensions up to 128")
+    _require(1 <= d <= 128, "Only supports head dimensions up to 128")
     nheads_k = k_cache.shape[2] if k_cache.ndim == 4 else 0
     _require(nheads == 0 or (nheads_k > 0 and nheads % nheads_k == 0), f"{nheads} query heads do not share {nheads_k} key heads evenly")
     _check_paged(k_cache, v_cache, page_table, lengths, batch, q, nheads_k)

@@ -266,6 +266,37 @@ def test_attention_leaves_out_bad_pages_and_cuts_lengths():
         assert lib.rgd_device_status() == 0
 
 
+@pytest.mark.parametrize("longest", [40, 3000])
+@pytest.mark.parametrize("entry", [-1, -2 ** 31, 2 ** 31 - 1, "pages"])
+def test_every_bad_entry_is_reported(longest, entry):
+    """One bad entry of a live page, in a table for few and for many keys; the same entry past the sequence is fine."""
+    lib = _lib.load()
+    assert lib.rgd_device_status() == 0
+    q, kc, vc, table, n = _case([longest, 33], 2, 2, 64, 16, "tokens", torch.float16, 21)
+    value = kc.shape[0] if entry == "pages" else entry
+    for at, status in ((2, _lib.RGD_E_PAGE), (3, 0)):
+        t = table.clone()
+        t[1, min(at, t.shape[1] - 1)] = value
+        if at < t.shape[1]:
+            o = F_.paged_attention_func(q.cuda(), kc.cuda(), vc.cuda(), t.cuda(), n.cuda())
+            P.assert_attention(o, None, P.attention(q, kc, vc, t, n, 64 ** -0.5), "o")
+            assert lib.rgd_device_status() == status
+
+
+def test_a_pool_without_pages():
+    lib = _lib.load()
+    q = randn(gen(22), 2, 1, 4, 64, dtype=torch.float16).cuda()
+    empty = torch.empty(0, 16, 2, 64, dtype=torch.float16, device="cuda")
+    table, n = torch.zeros(2, 200, dtype=torch.int32, device="cuda"), torch.tensor([3000, 5], dtype=torch.int32, device="cuda")
+    for t in (table, table[:, :1]):
+        o, lse = F_.paged_attention_func(q, empty, empty, t, n, return_lse=True)
+        assert (o == 0).all() and (lse == -math.inf).all()
+        assert lib.rgd_device_status() == _lib.RGD_E_PAGE
+    key = q[:, :, :2]
+    F_.paged_cache_append_fn(key, key, empty, empty, table, torch.zeros_like(n))
+    assert lib.rgd_device_status() == _lib.RGD_E_PAGE
+
+
 def test_attention_bias_of_the_types_lowest_value():
     """Buckets masked with -inf and with the lowest finite value; a row that is masked whole."""
     q, kc, vc, table, n = _case([100, 9], 2, 1, 64, 16, "tokens", torch.bfloat16, 9)

@@ -48,6 +48,7 @@ def test_slots_are_found_and_bad_pages_are_not_followed():
     assert at(c, 0, 127) == 0 and k.value == (2 ** 31 - 2) * 131072 + 127 * 1024
     assert at(_paged(table, 1 << 29), 0, 5) == _lib.RGD_E_SIZE           # positions are 31-bit
     assert at(_paged(table, 0), 0, 5) == _lib.RGD_E_INVALID
+    assert at(_paged(table, ss=-60), 0, 5) == _lib.RGD_E_STRIDE
 
 
 def test_c_abi_argument_checks():
