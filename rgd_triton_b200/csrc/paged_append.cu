@@ -6,6 +6,7 @@
 // Every input is read once and every output written once.
 #include "attn_mma.cuh"
 #include "paged.cuh"
+#include "sm100_prims.cuh"
 
 namespace rgd {
 namespace paged {
@@ -80,6 +81,8 @@ template <typename T, int VE>
 __global__ void __launch_bounds__(APPEND_THREADS, 4) append_kernel(const __grid_constant__ AppendParams p) {
     using V = Vec<T, VE>;
     extern __shared__ __align__(16) unsigned char raw[];
+    sm100::grid_trigger();
+    sm100::grid_wait();         // as the attention
     const int which = blockIdx.y, tid = threadIdx.x;
     const AppendGeo &g = p.geo[which == 2];
     const int heads = which == 2 ? p.Hq : p.Hkv, all = p.B * p.N, mine = g.loop * g.tokens;
@@ -235,9 +238,7 @@ int launch_append(AppendParams &p, cudaStream_t st) {
         const size_t bytes = (size_t)g.loop * g.tokens * (sizeof(Place) + angle_bytes);
         smem = bytes > smem ? bytes : smem;
     }
-    append_kernel<T, VE><<<dim3((unsigned)grid, p.Hq > 0 ? 3 : 2), APPEND_THREADS, smem, st>>>(p);
-    count_launch();
-    return check_launch();
+    return sm100::launch_pdl(append_kernel<T, VE>, dim3((unsigned)grid, p.Hq > 0 ? 3 : 2), APPEND_THREADS, smem, st, p);
 }
 
 int append_status_fetch() {

@@ -57,18 +57,19 @@ __device__ __forceinline__ int live_length(const AttnParams &p, int b, bool repo
 // Two forms in which the four warps of a CTA shared a unit were slower: with the maxima and weights of a tile exchanged
 // and the channels split, three barriers a tile held the loop (120 us for one sequence of 131 thousand keys, 93 us like
 // this); with 16 keys of a tile each, added up at the unit's end, short sequences paid for that (103 us for 64 of 16
-// to 8192 keys, 75 like this).
+// to 8192 keys, 72 like this).
 //
-// One B200, cold L2: 64 sequences of 16 to 8192 keys, 32 / 8 heads of 128 (366 MB) 75 us, one of 131 thousand (537 MB)
-// 97-104 us.  Once the rings are full the keys arrive at 6.8 TB/s; 7 us go by before (lengths, table entries and first
+// One B200, cold L2: 64 sequences of 16 to 8192 keys, 32 / 8 heads of 128 (366 MB) 72 us, one of 131 thousand (537 MB)
+// 97 us (104 on some of the GPUs).  Once the rings are full the keys arrive at 6.8 TB/s; 7 us go by before (lengths, table entries and first
 // tiles are reads that wait for one another), the warps end within 10 % of one another, and the join takes 3 us.
 //
 // Weights are split into two numbers of the cache's type (hi + lo): rounded to one, they would cost as much accuracy
 // as the output's own rounding, and the matrix pipe idles anyway.
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int WARPS = 4, THREADS = WARPS * 32, ROWS = 16, STAGES = 3, CTAS_PER_SM = 2;
-constexpr int UNIT_COST = 2;            // of a unit's queries and output, in tiles
-constexpr int MIN_COST = 3;             // least run of a warp
+// In tiles: what a unit's queries and output cost, and the least run of a warp.  us for 64 sequences of 16 to 8192 keys
+// with 8 cache heads / 48 of up to 2500 with 24: 71.6 / 35.8 like this, 72.2 / 36.9 at 2 and 3, 73.3 / 39.6 at 4 and 5.
+constexpr int UNIT_COST = 1, MIN_COST = 2;
 static_assert(MIN_COST > UNIT_COST, "a run that begins a unit has its first tile");
 
 __host__ __device__ constexpr int tile_keys(int D) { return D > 64 ? 16 : 32; }      // 8 KB of keys and values
@@ -150,6 +151,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attn_kernel(const __grid
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gq = lane >> 2, tq = lane & 3;
     const int warps = gridDim.x * WARPS, me = blockIdx.x * WARPS + warp;
     sm100::grid_trigger();
+    sm100::grid_wait();         // the launch may overlap the end of what ran before; nothing of that has been read so far
     auto tiles_of = [](int len) { return (len + KEYS - 1) / KEYS; };
     auto cost_of = [&](int tiles) { return tiles > 0 ? tiles + UNIT_COST : 0; };
 
@@ -671,6 +673,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const __grid_constan
     __shared__ float m_s[GROUPS], l_s[GROUPS];
     __shared__ float4 acc_s[GROUPS][QUADS];
     const int tid = threadIdx.x, quad = tid % QUADS, grp = tid / QUADS, row = blockIdx.y, warps = gridDim.x * WARPS;
+    sm100::grid_trigger();
     sm100::grid_wait();
     const Header *heads = reinterpret_cast<const Header *>(p.work) + blockIdx.x * WARPS;
     auto there = [&](const Header &head) { return head.last >= 0 && row < min(ROWS, p.G - head.row0); };
@@ -743,9 +746,7 @@ int launch(AttnParams &p, const Plan &plan, cudaStream_t st) {
     constexpr size_t smem = sizeof(Smem<T, D>);
     static_assert(CTAS_PER_SM * (smem + 1024) <= 228 << 10, "shared memory of an SM");
     if (int e = ensure_dyn_smem(reinterpret_cast<const void *>(kernel), smem)) return e;
-    kernel<<<plan.grid, THREADS, smem, st>>>(p);
-    count_launch();
-    if (int e = check_launch()) return e;
+    if (int e = sm100::launch_pdl(kernel, dim3(plan.grid), THREADS, smem, st, p)) return e;
     if (plan.direct) return RGD_OK;
     return sm100::launch_pdl(join_kernel<T, D>, dim3(plan.grid, (unsigned)(p.G < ROWS ? p.G : ROWS)), JOIN_THREADS, 0, st, p);
 }

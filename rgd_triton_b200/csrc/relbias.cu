@@ -46,6 +46,7 @@ __global__ void __launch_bounds__(FWD_THREADS) relbias_fwd_kernel(const __grid_c
     T *lut = reinterpret_cast<T *>(raw);                // [SHIFTS][L]: lut[s][x] = row[x + s]
     int *at = reinterpret_cast<int *>(raw + 16 * (size_t)L);
     T *w = reinterpret_cast<T *>(at + MAX_SIDE);
+    sm100::grid_wait();         // the launch may overlap the end of what ran before; nothing of that has been read so far
     const int h = blockIdx.z, i0 = blockIdx.y * p.rows, j0 = blockIdx.x * p.cols, tid = threadIdx.x;
     const int side = p.borders.side, both = p.borders.both;
     for (int k = tid; k < side - 1; k += FWD_THREADS) at[k] = p.borders.at[k];
@@ -130,6 +131,7 @@ __global__ void __launch_bounds__(BWD_THREADS, BWD_PER_SM) relbias_bwd_kernel(co
     extern __shared__ float hist[];                     // [BWD_WARPS][buckets]
     __shared__ int at[MAX_SIDE];
     sm100::grid_trigger();
+    sm100::grid_wait();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, h = blockIdx.y;
     const int side = p.borders.side, both = p.borders.both, buckets = side * (1 + both);
     const int row_chunk = blockIdx.x / p.across, m = blockIdx.x - row_chunk * p.across;
@@ -268,18 +270,17 @@ int launch_fwd(FwdParams &p, int H, cudaStream_t st) {
     p.rows = across * ceil_div64(p.Tq, 128) * H >= 2 * num_sms() ? 128 : 32;
     const size_t smem = fwd_smem<T>(p.rows, p.cols, p.borders.side * (1 + p.borders.both));
     static_assert(fwd_smem<T>(128, FWD_COLS, 2 * MAX_SIDE) <= 48 << 10, "more than a kernel gets without asking");
-    relbias_fwd_kernel<T><<<dim3((unsigned)across, (unsigned)ceil_div64(p.Tq, p.rows), (unsigned)H), FWD_THREADS, smem, st>>>(p);
-    count_launch();
-    return check_launch();
+    // Without a trigger for what follows, and so is the sum behind the gradient: gradient CTAs that wait on the SMs for a
+    // large forward to end cost it 90 us (24 x 4096 x 4096 and its gradient 294 -> 385 us).
+    return sm100::launch_pdl(relbias_fwd_kernel<T>, dim3((unsigned)across, (unsigned)ceil_div64(p.Tq, p.rows), (unsigned)H), FWD_THREADS, smem,
+                             st, p);
 }
 template <typename T>
 int launch_bwd(const BwdParams &p, const BwdGrid &grid, bool vec, cudaStream_t st) {
     const int buckets = p.borders.side * (1 + p.borders.both);
     const size_t smem = (size_t)BWD_WARPS * buckets * sizeof(float);
     auto kernel = vec ? relbias_bwd_kernel<T, true> : relbias_bwd_kernel<T, false>;
-    kernel<<<dim3((unsigned)grid.ctas, (unsigned)p.H), BWD_THREADS, smem, st>>>(p);
-    count_launch();
-    if (int e = check_launch()) return e;
+    if (int e = sm100::launch_pdl(kernel, dim3((unsigned)grid.ctas, (unsigned)p.H), BWD_THREADS, smem, st, p)) return e;
     return sm100::launch_pdl(relbias_sum_kernel, dim3((unsigned)buckets, (unsigned)p.H), BWD_THREADS, 0, st, p, grid.ctas);
 }
 
