@@ -113,6 +113,7 @@ struct Header {
 // A CTA whose runs lie inside one unit that ends behind them leaves one part, its first warp's.  So of a unit that ends
 // in another CTA, every CTA in between has one part, the last one a part per warp, the first one either.
 __host__ __device__ constexpr int64_t part_floats(int D) { return ROWS * (D + 2); }
+static_assert(WARPS * sizeof(Header) % 16 == 0, "parts lie behind the headers, on 16 bytes");
 __host__ __device__ __forceinline__ int64_t workspace_bytes(int ctas, int D) {
     return (int64_t)ctas * WARPS * ((int64_t)sizeof(Header) + 2 * part_floats(D) * (int64_t)sizeof(float));
 }

@@ -152,3 +152,37 @@ def test_position_bias_module():
     sig = lambda f: list(inspect.signature(f).parameters)
     assert sig(ops.RelativePositionBias.forward) == ["self", "seqlen_q", "seqlen_k", "offset", "dtype"]
     assert sig(ops.PagedAttention.forward) == ["self", "q", "k_cache", "v_cache", "page_table", "lengths", "softmax_scale", "rel_bias"]
+
+
+def test_registered_operators_give_the_kernels_shapes():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    from rgd_triton_b200 import library  # noqa: F401
+    bf = torch.bfloat16
+    with FakeTensorMode():
+        w = torch.empty(32, 5, device="cuda")
+        b = torch.ops.rgd_b200.relbias(w, 10, 21, True, 128, 0, bf)
+        assert b.shape == (1, 5, 10, 21) and b.dtype == bf and b.stride() == (5 * 10 * 24, 10 * 24, 24, 1)
+        dw = torch.ops.rgd_b200.relbias_bwd(b, 32, True, 128, 0, torch.float32)
+        assert dw.shape == w.shape and dw.dtype == w.dtype
+        kc = torch.empty(7, 16, 2, 64, device="cuda", dtype=bf)
+        table, n = torch.empty(3, 4, device="cuda", dtype=torch.int32), torch.empty(3, device="cuda", dtype=torch.int32)
+        key, q = torch.empty(3, 9, 2, 64, device="cuda", dtype=bf), torch.empty(3, 9, 8, 64, device="cuda", dtype=bf)
+        pos = torch.empty(2, 64, 32, device="cuda")
+        assert torch.ops.rgd_b200.paged_append(key, key, kc, kc, table, n, pos, q, None).shape == q.shape
+        assert torch.ops.rgd_b200.paged_append(key, key, kc, kc, table, n, None, None, n).numel() == 0
+        o, lse = torch.ops.rgd_b200.paged_attn(q[:, :1], kc, kc, table, n, None, None, False, 128)
+        assert o.shape == (3, 1, 8, 64) and o.dtype == bf and lse.shape == (3, 8) and lse.dtype == torch.float32
+
+
+def test_workspaces_follow_the_plan():
+    """None where every unit has a CTA, a part of a 16-row tile for every warp otherwise, refusals past 32-bit schedules."""
+    lib = _lib.load()
+    size = lambda B, Hq, Hk, d, pages, page: lib.rgd_paged_attn_workspace_bytes(B, Hq, Hk, d, pages, page)
+    assert size(1, 16, 16, 128, 19, 16) == 0 and size(16, 16, 16, 64, 28, 32) == 0
+    per_warp = lambda D: 20 + 2 * 16 * (D + 2) * 4
+    for args, D in (((1, 1, 1, 128, 64, 16), 128), ((64, 24, 24, 64, 1000, 16), 64), ((1, 32, 8, 96, 5000, 24), 128)):
+        assert size(*args) > 0 and size(*args) % (4 * per_warp(D)) == 0
+    assert size(1 << 20, 64, 64, 128, 1 << 16, 16) == _lib.RGD_E_SIZE
+    assert size(4, 5, 2, 64, 4, 16) == _lib.RGD_E_INVALID and size(4, 0, 0, 64, 4, 16) == 0
+
