@@ -141,7 +141,11 @@ struct FastDiv {
     uint32_t mul, shr, div;
 };
 __host__ __device__ __forceinline__ uint32_t fdiv(uint32_t n, const FastDiv &f) {
+#ifdef __CUDA_ARCH__
+    return f.div == 1 ? n : (__umulhi(n, f.mul) >> f.shr);
+#else
     return f.div == 1 ? n : ((uint32_t)(((uint64_t)n * f.mul) >> 32) >> f.shr);
+#endif
 }
 static inline FastDiv make_fastdiv(uint32_t d) {
     FastDiv f{0, 0, d};
