@@ -25,16 +25,18 @@ struct FwdParams {
     void *out;
     int64_t o_sh, o_sq;
     int Tq, Tk, offset;
-    int rows, cols;             // of a tile; both multiples of 8
+    int cols;                   // of a tile, a multiple of 8
+    FastDiv across;             // tiles side by side
 };
 
-constexpr int FWD_THREADS = 256;
-constexpr int FWD_COLS = 2048;
+// Tiles of 32 rows: small ones end together.  us for 24 x 4096 x 4096 fp16 and its gradient at 32, 48, 64, 128 rows:
+// 251, 253, 258, 265.
+constexpr int FWD_THREADS = 256, FWD_ROWS = 32, FWD_COLS = 2048;
 
 // Shared memory: the short row (tile cols + rows values, rounded up) at each shift, the borders, the head's weights.
-template <typename T> __host__ __device__ constexpr int fwd_row_values(int rows, int cols) { return rows + cols + 16 / (int)sizeof(T); }
-template <typename T> constexpr size_t fwd_smem(int rows, int cols, int buckets) {
-    return 16 * (size_t)fwd_row_values<T>(rows, cols) + MAX_SIDE * sizeof(int) + (size_t)buckets * sizeof(T);
+template <typename T> __host__ __device__ constexpr int fwd_row_values(int cols) { return FWD_ROWS + cols + 16 / (int)sizeof(T); }
+template <typename T> constexpr size_t fwd_smem(int cols, int buckets) {
+    return 16 * (size_t)fwd_row_values<T>(cols) + MAX_SIDE * sizeof(int) + (size_t)buckets * sizeof(T);
 }
 
 template <typename T>
@@ -42,18 +44,19 @@ __global__ void __launch_bounds__(FWD_THREADS) relbias_fwd_kernel(const __grid_c
     constexpr int SHIFTS = 16 / sizeof(T);
     using V = Vec<T, SHIFTS>;
     extern __shared__ __align__(16) unsigned char raw[];
-    const int L = fwd_row_values<T>(p.rows, p.cols);
+    const int L = fwd_row_values<T>(p.cols);
     T *lut = reinterpret_cast<T *>(raw);                // [SHIFTS][L]: lut[s][x] = row[x + s]
     int *at = reinterpret_cast<int *>(raw + 16 * (size_t)L);
     T *w = reinterpret_cast<T *>(at + MAX_SIDE);
     sm100::grid_wait();         // the launch may overlap the end of what ran before; nothing of that has been read so far
-    const int h = blockIdx.z, i0 = blockIdx.y * p.rows, j0 = blockIdx.x * p.cols, tid = threadIdx.x;
+    const int down = (int)fdiv(blockIdx.x, p.across), h = blockIdx.y, tid = threadIdx.x;
+    const int i0 = down * FWD_ROWS, j0 = ((int)blockIdx.x - down * (int)p.across.div) * p.cols;
     const int side = p.borders.side, both = p.borders.both;
     for (int k = tid; k < side - 1; k += FWD_THREADS) at[k] = p.borders.at[k];
     for (int k = tid; k < side * (1 + both); k += FWD_THREADS) w[k] = from_f32<T>(load_as_f32(p.w, k * p.w_sk + h * p.w_sh, p.w_dtype));
     __syncthreads();
-    // row[x] belongs to j - i = (j0 - i0) - (rows - 1) + x: row r of the tile begins at x = rows - 1 - r
-    const int first = j0 - i0 - (p.rows - 1) - p.offset;
+    // row[x] belongs to j - i = (j0 - i0) - (FWD_ROWS - 1) + x: row r of the tile begins at x = FWD_ROWS - 1 - r
+    const int first = j0 - i0 - (FWD_ROWS - 1) - p.offset;
     for (int x = tid; x < L; x += FWD_THREADS) lut[x] = w[bucket_of(at, side, both, first + x)];
     __syncthreads();
     for (int x = tid * SHIFTS; x + SHIFTS < L; x += FWD_THREADS * SHIFTS) {
@@ -68,10 +71,10 @@ __global__ void __launch_bounds__(FWD_THREADS) relbias_fwd_kernel(const __grid_c
     }
     sm100::fence_proxy_async_smem();
     __syncthreads();
-    const int rows = min(p.rows, p.Tq - i0), cols = min(p.cols, p.Tk - j0), even = cols / SHIFTS * SHIFTS;
+    const int rows = min(FWD_ROWS, p.Tq - i0), cols = min(p.cols, p.Tk - j0), even = cols / SHIFTS * SHIFTS;
     T *out = reinterpret_cast<T *>(p.out) + (int64_t)h * p.o_sh + (int64_t)i0 * p.o_sq + j0;
     for (int r = tid; r < rows; r += FWD_THREADS) {
-        const int x = p.rows - 1 - r, s = x % SHIFTS;
+        const int x = FWD_ROWS - 1 - r, s = x % SHIFTS;
         if (even > 0) sm100::bulk_store_1d(out + (int64_t)r * p.o_sq, lut + s * L + (x - s), (uint32_t)(even * sizeof(T)));
         for (int j = even; j < cols; ++j) out[(int64_t)r * p.o_sq + j] = lut[x + j];
     }
@@ -245,35 +248,31 @@ __global__ void __launch_bounds__(BWD_THREADS) relbias_sum_kernel(const __grid_c
         store_from_f32(p.dw, (int64_t)b * p.H + h, p.w_dtype, (float)((warp_sum[0] + warp_sum[1]) + (warp_sum[2] + warp_sum[3])));
 }
 
-// Rows of a CTA: few for small problems, so that they spread over the chip.
+// Rows of a CTA: 64, few enough for the last CTAs to end together (24 x 4096 x 4096 fp16 and its bias at 64, 128, 256, 512
+// rows: 265, 273, 292, 337 us); 32 for problems that leave room on the chip.
 struct BwdGrid {
     int chunk, across, ctas;
 };
 BwdGrid bwd_grid(int64_t H, int64_t Tq, int64_t Tk) {
     const int64_t nI = (Tq + 7) / 8, nJ = (Tk + 7) / 8;
-    int chunk = 32;
-    auto across = [&] { return ceil_div64(nJ + chunk - 1, BWD_THREADS); };
-    auto ctas = [&] { return ceil_div64(nI, chunk) * across(); };
-    for (; chunk > 4; chunk /= 2) {         // as few as still leave one wave
-        const int64_t half = ceil_div64(nI, chunk / 2) * ceil_div64(nJ + chunk / 2 - 1, BWD_THREADS);
-        if (H * half > BWD_PER_SM * num_sms()) break;
-    }
-    return {chunk, (int)across(), (int)ctas()};
+    auto grid = [&](int chunk) {
+        const int64_t across = ceil_div64(nJ + chunk - 1, BWD_THREADS);
+        return BwdGrid{chunk, (int)across, (int)(across * ceil_div64(nI, chunk))};
+    };
+    const BwdGrid fine = grid(4);
+    return H * fine.ctas <= BWD_PER_SM * num_sms() ? fine : grid(8);
 }
 
 template <typename T>
 int launch_fwd(FwdParams &p, int H, cudaStream_t st) {
-    // Tiles of 128 rows spread the evaluation of the short row over 128 of its windows; problems that would not fill
-    // the chip with them take 32.
     p.cols = (int)(p.Tk < FWD_COLS ? (p.Tk + 7) / 8 * 8 : FWD_COLS);
-    const int64_t across = ceil_div64(p.Tk, p.cols);
-    p.rows = across * ceil_div64(p.Tq, 128) * H >= 2 * num_sms() ? 128 : 32;
-    const size_t smem = fwd_smem<T>(p.rows, p.cols, p.borders.side * (1 + p.borders.both));
-    static_assert(fwd_smem<T>(128, FWD_COLS, 2 * MAX_SIDE) <= 48 << 10, "more than a kernel gets without asking");
+    const int64_t across = ceil_div64(p.Tk, p.cols), ctas = across * ceil_div64(p.Tq, FWD_ROWS);
+    p.across = make_fastdiv((uint32_t)across);
+    const size_t smem = fwd_smem<T>(p.cols, p.borders.side * (1 + p.borders.both));
+    static_assert(fwd_smem<T>(FWD_COLS, 2 * MAX_SIDE) <= 48 << 10, "more than a kernel gets without asking");
     // Without a trigger for what follows, and so is the sum behind the gradient: gradient CTAs that wait on the SMs for a
     // large forward to end cost it 90 us (24 x 4096 x 4096 and its gradient 294 -> 385 us).
-    return sm100::launch_pdl(relbias_fwd_kernel<T>, dim3((unsigned)across, (unsigned)ceil_div64(p.Tq, p.rows), (unsigned)H), FWD_THREADS, smem,
-                             st, p);
+    return sm100::launch_pdl(relbias_fwd_kernel<T>, dim3((unsigned)ctas, (unsigned)H), FWD_THREADS, smem, st, p);
 }
 template <typename T>
 int launch_bwd(const BwdParams &p, const BwdGrid &grid, bool vec, cudaStream_t st) {
