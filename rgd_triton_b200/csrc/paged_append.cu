@@ -73,7 +73,7 @@ struct alignas(16) Place {
 // Each CTA has one of the three tensors and a few tokens of it, each thread one group of VE channels (16 bytes, or a
 // pair where views are not addressable that way) of one head after another.  Where the tokens go and their angles are
 // looked up once for the CTA, two dependent reads (length; table entry and angles) during which the first tokens are on
-// their way; the loop is then read, turn, write.  [4, 4096, 16, 128] bf16 keys, values and queries (411 MB): 76 us, 83 %
+// their way; the loop is then read, turn, write.  [4, 4096, 16, 128] bf16 keys, values and queries (411 MB): 77 us, 81 %
 // of the copy rate, bound by instruction issue (two thirds of the slots busy) and the look-ups.  With every thread
 // looking up its own tokens it executed 222 instructions per 16 bytes instead of 130 and took 160-200 us.  Four CTAs an
 // SM: at five the registers spill (84 us).
@@ -226,12 +226,13 @@ int launch_append(AppendParams &p, cudaStream_t st) {
         g.tokens = APPEND_THREADS / g.per_token;
         g.by_per_token = make_fastdiv((uint32_t)g.per_token);
         // Tokens one after another: the look-ups of a CTA are worth about as much as two tokens (4 x 4096 tokens of 48
-        // heads: 180 us at one, 113 at two, 86 at four, 78 at eight, 80 at sixteen), but every SM should have four
-        // CTAs, and the angles have to fit.
+        // heads: 180 us at one, 113 at two, 86 at four, 77 at eight, 80 at sixteen), but every SM should have four
+        // CTAs, sixteen for a second batch of reads (7 ragged sequences of up to 333 tokens: 7.6 us at eight, 6.7 at
+        // four), and the angles have to fit.
         const int64_t batches = ceil_div64(all, g.tokens), spread = batches * (p.Hq > 0 ? 3 : 2) / (4 * num_sms());
         const size_t angle_bytes = (size_t)p.angle_groups * 16 * sizeof(float);
         const int64_t fit = p.R > 0 ? (int64_t)(ANGLE_BYTES / (g.tokens * angle_bytes)) : APPEND_LOOP;
-        const int64_t loop = spread < fit ? spread : fit;
+        const int64_t want = spread < 4 * APPEND_BATCH && spread > APPEND_BATCH ? APPEND_BATCH : spread, loop = want < fit ? want : fit;
         g.loop = (int)(loop < 1 ? 1 : loop > APPEND_LOOP ? APPEND_LOOP : loop);
         const int64_t ctas = ceil_div64(batches, g.loop);
         grid = ctas > grid ? ctas : grid;
