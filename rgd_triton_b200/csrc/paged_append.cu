@@ -70,21 +70,27 @@ struct alignas(16) Place {
     int position;                           // -1: a key or value that is not written, a query that is copied
 };
 
+// A pair of channels as two floats.
+template <typename T> __device__ __forceinline__ float2 unpack(uint32_t w);
+template <> __device__ __forceinline__ float2 unpack<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2 *>(&w)); }
+template <> __device__ __forceinline__ float2 unpack<__nv_bfloat16>(uint32_t w) {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+
 // Each CTA has one of the three tensors and a few tokens of it, each thread one group of VE channels (16 bytes, or a
 // pair where views are not addressable that way) of one head after another.  Where the tokens go and their angles are
 // looked up once for the CTA, two dependent reads (length; table entry and angles) during which the first tokens are on
-// their way; the loop is then read, turn, write.  [4, 4096, 16, 128] bf16 keys, values and queries (411 MB): 77 us, 81 %
+// their way; the loop is then read, turn, write.  [4, 4096, 16, 128] bf16 keys, values and queries (411 MB): 73 us, 86 %
 // of the copy rate, bound by instruction issue (two thirds of the slots busy) and the look-ups.  With every thread
-// looking up its own tokens it executed 222 instructions per 16 bytes instead of 130 and took 160-200 us.  Four CTAs an
-// SM: at five the registers spill (84 us).
+// looking up its own tokens it took 160-200 us.  Four CTAs an SM: 74 us at five, and ragged sequences 6.6 us for 6.0.
 template <typename T, int VE>
 __global__ void __launch_bounds__(APPEND_THREADS, 4) append_kernel(const __grid_constant__ AppendParams p) {
-    using V = Vec<T, VE>;
+    using V = Vec<uint32_t, VE / 2>;            // pairs of channels
     extern __shared__ __align__(16) unsigned char raw[];
     sm100::grid_trigger();
     sm100::grid_wait();         // as the attention
     const int which = blockIdx.y, tid = threadIdx.x;
-    const AppendGeo &g = p.geo[which == 2];
+    const AppendGeo g = p.geo[which == 2];      // a copy: an indexed parameter is read anew at every use (77 us for 73)
     const int heads = which == 2 ? p.Hq : p.Hkv, all = p.B * p.N, mine = g.loop * g.tokens;
     if (heads == 0 || (int64_t)blockIdx.x * mine >= all) return;       // the grid is the larger one of two
     const int first = blockIdx.x * mine;
@@ -110,10 +116,10 @@ __global__ void __launch_bounds__(APPEND_THREADS, 4) append_kernel(const __grid_
         for (int u = 0; u < APPEND_BATCH; ++u) {
             if (t0 + u < g.loop && token < all) {
                 if constexpr (VE == 8) {
-                    v[u] = load_vec_stream<T, VE>(from);
+                    v[u] = load_vec_stream<uint32_t, 4>(reinterpret_cast<const uint32_t *>(from));
                 } else {
-                    v[u].v[0] = from[0];
-                    v[u].v[1] = c + 1 < p.d ? from[1] : from_f32<T>(0.f);
+                    const T pair[2] = {from[0], c + 1 < p.d ? from[1] : from_f32<T>(0.f)};
+                    v[u].v[0] = (uint32_t)reinterpret_cast<const uint16_t *>(pair)[0] | (uint32_t)reinterpret_cast<const uint16_t *>(pair)[1] << 16;
                 }
             }
             token += g.tokens;
@@ -190,18 +196,19 @@ __global__ void __launch_bounds__(APPEND_THREADS, 4) append_kernel(const __grid_
 #pragma unroll
                         for (int k = 0; k < (VE == 8 ? 4 : 2); k += 2) {
                             if (e + k >= rotated) break;            // R is even: a rotated pair is whole
-                            const float x0 = to_f32<T>(v[u].v[e + k]), x1 = to_f32<T>(v[u].v[e + k + 1]);
-                            *reinterpret_cast<uint32_t *>(&v[u].v[e + k]) =
-                                attn::Mma<T>::pack(x0 * cw.v[k] - x1 * sw.v[k], x1 * cw.v[k + 1] + x0 * sw.v[k + 1]);
+                            uint32_t &pair = v[u].v[(e + k) / 2];
+                            const float2 x = unpack<T>(pair);
+                            pair = attn::Mma<T>::pack(x.x * cw.v[k] - x.y * sw.v[k], x.y * cw.v[k + 1] + x.x * sw.v[k + 1]);
                         }
                     }
                 }
                 T *to = out_row + at.out;
                 if constexpr (VE == 8) {
-                    store_vec<T, VE>(to, v[u]);
+                    store_vec<uint32_t, 4>(reinterpret_cast<uint32_t *>(to), v[u]);
                 } else {
-                    to[0] = v[u].v[0];
-                    if (c + 1 < p.d) to[1] = v[u].v[1];
+                    const uint16_t lo = (uint16_t)v[u].v[0], hi = (uint16_t)(v[u].v[0] >> 16);
+                    reinterpret_cast<uint16_t *>(to)[0] = lo;
+                    if (c + 1 < p.d) reinterpret_cast<uint16_t *>(to)[1] = hi;
                 }
             }
         }
@@ -226,9 +233,9 @@ int launch_append(AppendParams &p, cudaStream_t st) {
         g.tokens = APPEND_THREADS / g.per_token;
         g.by_per_token = make_fastdiv((uint32_t)g.per_token);
         // Tokens one after another: the look-ups of a CTA are worth about as much as two tokens (4 x 4096 tokens of 48
-        // heads: 180 us at one, 113 at two, 86 at four, 77 at eight, 80 at sixteen), but every SM should have four
-        // CTAs, sixteen for a second batch of reads (7 ragged sequences of up to 333 tokens: 7.6 us at eight, 6.7 at
-        // four), and the angles have to fit.
+        // heads: 168 us at one, 107 at two, 81 at four, 73 at eight, 74 at sixteen), but every SM should have four
+        // CTAs, sixteen for a second batch of reads (7 ragged sequences of up to 333 tokens: 6.0 us with this rule,
+        // 6.9 without it), and the angles have to fit.
         const int64_t batches = ceil_div64(all, g.tokens), spread = batches * (p.Hq > 0 ? 3 : 2) / (4 * num_sms());
         const size_t angle_bytes = (size_t)p.angle_groups * 16 * sizeof(float);
         const int64_t fit = p.R > 0 ? (int64_t)(ANGLE_BYTES / (g.tokens * angle_bytes)) : APPEND_LOOP;
