@@ -393,7 +393,7 @@ int64_t rgd_relbias_bwd_workspace_bytes(int64_t H, int64_t Tq, int64_t Tk,
                                         int num_buckets);
 /* dweight[k, h] = sum of dbias[h, i, j] over bucket(j - i - offset) = k, in a
  * fixed order, rounded once to bias->dtype.  dbias: [H, Tq, Tk] of dtype
- * through element strides (any, 0 included), unit key stride.  dweight: dense
+ * through element strides (0 included), unit key stride.  dweight: dense
  * [num_buckets, H].  bias->weight and its strides are not used. */
 int rgd_relbias_bwd(const rgd_relbias *bias, const void *dbias,
                     int64_t stride_h, int64_t stride_q, int dtype,
@@ -460,10 +460,10 @@ int64_t rgd_paged_attn_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv,
  * adds weight[bucket(lengths[b] - 1 - j), h].  lse (NULL or fp32 [B, Hq]):
  * log-sum-exp.  A sequence of length 0 gets zeros and lse -inf; so does one
  * without a usable page.  Keys of pages out of range are left out.  dtype
- * RGD_F16 / RGD_BF16, d <= 128, Hq a multiple of Hkv, B * Hkv * ceil(Hq / Hkv /
- * 16) * (max_pages * page_size / 16 + 3) below 2^31.  The order of all sums
- * depends on the lengths, max_pages, page_size and the device, not on the run:
- * results are bit-reproducible. */
+ * RGD_F16 / RGD_BF16, d <= 128, Hq a multiple of Hkv, B <= 2^30, B * Hkv *
+ * ceil(Hq / Hkv / 16) * (max_pages * page_size / 16 + 3) below 2^31.  The order
+ * of all sums depends on the lengths, max_pages, page_size and the device, not on
+ * the run: results are bit-reproducible. */
 int rgd_paged_attn(const rgd_heads *q, const rgd_paged *cache,
                    const rgd_relbias *bias, const rgd_heads *o, float *lse,
                    int64_t B, int64_t Hq, int64_t Hkv, int64_t d,

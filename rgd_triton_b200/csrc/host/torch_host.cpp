@@ -1053,6 +1053,7 @@ PyObject *py_paged_append(PyObject *, PyObject *const *args, Py_ssize_t n) {
         for (const Tensor *t : {&kc, &vc})
             for (int i = 0; i < 3; ++i)
                 if (t->size(i) > 1 && t->stride(i) <= 0) Py_RETURN_NONE;
+        if (c.k == c.v) Py_RETURN_NONE;
         const int64_t B = key.size(0), N = key.size(1), Hkv = key.size(2), d = key.size(3);
         int64_t P = 0, R = 0;
         if (pos.defined()) {

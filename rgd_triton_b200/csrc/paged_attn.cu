@@ -779,7 +779,7 @@ using namespace rgd;
 extern "C" int64_t rgd_paged_attn_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t d, int64_t max_pages, int64_t page_size) {
     if (B < 0 || Hq < 0 || Hkv < 0 || d < 0 || max_pages < 0 || page_size < 1) return RGD_E_INVALID;
     if (Hkv == 0 || Hq % Hkv != 0) return Hq == 0 ? 0 : RGD_E_INVALID;
-    if (d > 128 || B > INT32_MAX || Hq > 65535 || max_pages > INT32_MAX || page_size > INT32_MAX) return RGD_E_SIZE;
+    if (d > 128 || B > 1 << 30 || Hq > 65535 || max_pages > INT32_MAX || page_size > INT32_MAX) return RGD_E_SIZE;
     const int D = d > 64 ? 128 : 64;
     const int64_t units = Hkv * ceil_div64(Hq / Hkv, paged::ROWS);
     if (paged::too_large(B, units, max_pages * page_size, D)) return RGD_E_SIZE;
@@ -793,7 +793,7 @@ extern "C" int rgd_paged_attn(const rgd_heads *q, const rgd_paged *cache, const 
     if (!q || !o) return RGD_E_NULL;
     if (dtype != RGD_F16 && dtype != RGD_BF16) return RGD_E_DTYPE;
     if (B < 0 || Hq < 0 || Hkv < 0 || d < 0) return RGD_E_INVALID;
-    if (d > 128 || B > INT32_MAX || Hq > 65535) return RGD_E_SIZE;
+    if (d > 128 || B > 1 << 30 || Hq > 65535) return RGD_E_SIZE;
     if (Hq > 0 && (Hkv == 0 || Hq % Hkv != 0)) return RGD_E_INVALID;
     if (int e = paged::check_paged(cache, B, Hkv > 0 && d > 0)) return e;
     if (bias)

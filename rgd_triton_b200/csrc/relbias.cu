@@ -328,6 +328,7 @@ extern "C" int rgd_relbias_bwd(const rgd_relbias *bias, const void *dbias, int64
     if (int e = relbias::check(bias)) return e;
     if (!dtype_ok(dtype)) return RGD_E_DTYPE;
     if (int e = relbias::check_sizes(H, Tq, Tk, offset)) return e;
+    if (stride_h < 0 || stride_q < 0) return RGD_E_STRIDE;
     if (H == 0) return RGD_OK;
     if (!dweight || (!dbias && Tq > 0 && Tk > 0)) return RGD_E_NULL;
     cudaStream_t st = (cudaStream_t)stream;

@@ -1246,6 +1246,7 @@ def _append_launch(key, value, k_cache, v_cache, page_table, lengths, pos_emb, q
     _check_paged(k_cache, v_cache, page_table, lengths, batch, key, nheads_k)
     for c, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
         _require(all(s > 0 for s, size in zip(c.stride(), c.shape) if size > 1), f"{name} is written: its slots must not share memory")
+    _require(k_cache.data_ptr() != v_cache.data_ptr() or k_cache.numel() == 0, "k_cache and v_cache are written: they must not share memory")
     if counts is not None:
         _require(counts.ndim == 1 and counts.shape[0] == batch, f"counts must be ({batch},), got {tuple(counts.shape)}")
         _check_ints(key, counts=counts)

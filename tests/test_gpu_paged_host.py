@@ -191,3 +191,11 @@ def test_compiled_autograd_traces_the_backward():
     with torch._dynamo.compiled_autograd._enable(torch.compile(backend="aot_eager")):
         out.backward(dy)
     assert torch.equal(w.grad, want)
+
+
+def test_one_tensor_for_both_caches_is_refused_and_left_alone():
+    (k, v, _), kc, _, table, lengths, *_ = _step()
+    before = kc.clone()
+    with pytest.raises(AssertionError, match="share memory"):
+        F_.paged_cache_append_fn(k, v, kc, kc, table, lengths)
+    assert torch.equal(kc, before)

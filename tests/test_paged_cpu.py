@@ -186,3 +186,21 @@ def test_workspaces_follow_the_plan():
     assert size(1 << 20, 64, 64, 128, 1 << 16, 16) == _lib.RGD_E_SIZE
     assert size(4, 5, 2, 64, 4, 16) == _lib.RGD_E_INVALID and size(4, 0, 0, 64, 4, 16) == 0
 
+
+
+def test_one_tensor_for_both_caches_is_refused():
+    both = torch.zeros(5, 16, 4, 64, dtype=torch.bfloat16)
+    with pytest.raises(AssertionError, match="share memory"):
+        F_.paged_cache_append_fn(**_append_args(k_cache=both, v_cache=both))
+
+
+def test_c_abi_refuses_negative_gradient_strides_and_too_many_sequences():
+    lib = _lib.load()
+    borders = (C.c_int32 * 3)(1, 5, 9)
+    bias = C.byref(_lib.RelBias(1, 4, 1, 0, 4, 0, borders))
+    for sh, sq in ((-64, 8), (64, -8)):
+        assert lib.rgd_relbias_bwd(bias, 16, sh, sq, 0, 16, 4, 8, 8, 0, 16, 1 << 20, None) == _lib.RGD_E_STRIDE
+    h = C.byref(_lib.Heads(1, 8, 8, 8))
+    cache = _paged(torch.zeros(1, 0, dtype=torch.int32))                # no page: nothing else bounds the sequences
+    assert lib.rgd_paged_attn(h, C.byref(cache), None, h, None, (1 << 30) + 1, 1, 1, 64, 1.0, _lib.RGD_F16, None, 0, None) == _lib.RGD_E_SIZE
+    assert lib.rgd_paged_attn_workspace_bytes((1 << 30) + 1, 1, 1, 64, 0, 16) == _lib.RGD_E_SIZE
