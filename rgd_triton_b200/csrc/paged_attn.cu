@@ -84,11 +84,8 @@ struct Smem {
     };
     Stage ring[WARPS][STAGES];
     int64_t row[WARPS][2][2 * KEYS];                    // of the tiles to load next: element offsets of keys, of values; -1: none
-    int sums[WARPS], counts[WARPS];
-    struct Boundary {                                   // where a warp's run begins
-        int tiles;                                      // of all units before it
-        int b, unit, tile;
-    } at[WARPS + 1];
+    int upto[THREADS], filled[THREADS];                 // costs and sequences with a token, of a warp's threads up to each
+    int unit, tile;                                     // where the CTA's runs begin
     int borders[relbias::MAX_SIDE];                     // with a position bias
 };
 
@@ -178,69 +175,84 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attn_kernel(const __grid
     } else {
         // cost of a head's units before each sequence: every thread sums a run of sequences, then the runs are added up
         const int chunk = (p.B + THREADS - 1) / THREADS, b0 = min(tid * chunk, p.B), b1 = min(b0 + chunk, p.B);
-        int mine = 0, filled = 0;                               // cost; sequences with a token
+        int upto = 0, filled = 0;                               // cost; sequences with a token
         for (int b = b0; b < b1; ++b) {
             const int tiles = tiles_of(live_length(p, b, blockIdx.x == 0));
-            mine += cost_of(tiles);
+            upto += cost_of(tiles);
             filled += tiles > 0;
         }
-        int upto = mine, filled_upto = filled;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int x = __shfl_up_sync(0xffffffffu, upto, o), y = __shfl_up_sync(0xffffffffu, filled_upto, o);
+            const int x = __shfl_up_sync(0xffffffffu, upto, o), y = __shfl_up_sync(0xffffffffu, filled, o);
             if (lane >= o) {
                 upto += x;
-                filled_upto += y;
+                filled += y;
             }
         }
-        if (lane == 31) {
-            sm.sums[warp] = upto;
-            sm.counts[warp] = filled_upto;
-        }
+        sm.upto[tid] = upto;
+        sm.filled[tid] = filled;
         __syncthreads();
-        int all = 0;
+        int all = 0, all_filled = 0;
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) {
-            if (w < warp) {
-                upto += sm.sums[w];
-                filled_upto += sm.counts[w];
-            }
-            all += sm.sums[w];
+            all += sm.upto[w * 32 + 31];
+            all_filled += sm.filled[w * 32 + 31];
         }
         runs = Runs(all * p.units, warps);
-        // the boundaries of this CTA's runs: the thread whose sequences a boundary lies in finds it.  A unit's cost comes
-        // before its tiles.
+        // Where the CTA's runs begin and end, a lane per boundary, every warp for itself: the thread whose sequences hold
+        // the boundary by bisection, then the sequence.  A unit's cost comes before its tiles.
+        const int pos = runs.begin((int)blockIdx.x * WARPS + min(lane, WARPS));
+        int tiles_before = (all - all_filled * UNIT_COST) * p.units;    // of all units
+        int b_at = p.B, unit_at = 0, tile_at = 0, len_at = 0;
+        if (pos < runs.total) {
+            const int cost_at = (int)((unsigned)pos / (unsigned)p.units);
+            int t = 0, before = 0, filled_before = 0;
 #pragma unroll
-        for (int w = 0; w <= WARPS; ++w) {
-            const int pos = runs.begin((int)blockIdx.x * WARPS + w);
-            int before = upto - mine, filled_before = filled_upto - filled;
-            if (pos >= before * p.units && pos < upto * p.units) {
-                for (int b = b0; b < b1; ++b) {
-                    const int tiles = tiles_of(live_length(p, b, false)), cost = cost_of(tiles);
-                    if (pos < (before + cost) * p.units) {
-                        const int in = pos - before * p.units, unit = (int)((unsigned)in / (unsigned)cost), tile = max(in - unit * cost - UNIT_COST, 0);
-                        sm.at[w] = {(before - filled_before * UNIT_COST) * p.units + unit * tiles + tile, b, unit, tile};
-                        break;
-                    }
-                    before += cost;
-                    filled_before += tiles > 0;
+            for (int w = 0; w < WARPS - 1; ++w)
+                if (t == w * 32 && cost_at >= before + sm.upto[w * 32 + 31]) {
+                    before += sm.upto[w * 32 + 31];
+                    filled_before += sm.filled[w * 32 + 31];
+                    t += 32;
                 }
-            } else if (tid == THREADS - 1 && pos >= runs.total) {
-                sm.at[w] = {(all - filled_upto * UNIT_COST) * p.units, p.B, 0, 0};
+            int in_warp = 0;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1)
+                if (cost_at >= before + sm.upto[t + in_warp + o - 1]) in_warp += o;
+            if (in_warp > 0) {
+                before += sm.upto[t + in_warp - 1];
+                filled_before += sm.filled[t + in_warp - 1];
+            }
+            t += in_warp;
+            for (int b = t * chunk; b < min((t + 1) * chunk, p.B); ++b) {
+                const int len = live_length(p, b, false), tiles = tiles_of(len), cost = cost_of(tiles);
+                if (cost_at < before + cost) {
+                    const int in = pos - before * p.units;
+                    b_at = b;
+                    len_at = len;
+                    unit_at = (int)((unsigned)in / (unsigned)cost);
+                    tile_at = max(in - unit_at * cost - UNIT_COST, 0);
+                    tiles_before = (before - filled_before * UNIT_COST) * p.units + unit_at * tiles + tile_at;
+                    break;
+                }
+                before += cost;
+                filled_before += tiles > 0;
             }
         }
-        __syncthreads();
-        n = sm.at[warp + 1].tiles - sm.at[warp].tiles;
-        if (lane == 0) reinterpret_cast<Header *>(p.work)[me].last = -1;
-        merge = sm.at[0].b < p.B && sm.at[0].b == sm.at[WARPS].b && sm.at[0].unit == sm.at[WARPS].unit;
-        if (n > 0) {
-            at.b = sm.at[warp].b;
-            at.len = live_length(p, at.b, false);
-            at.tiles = tiles_of(at.len);
-            at.tile = sm.at[warp].tile;
-            at.hk = (int)fdiv((uint32_t)sm.at[warp].unit, p.by_groups);
-            at.group = sm.at[warp].unit - at.hk * p.groups;
+        auto of = [](int x, int boundary) { return __shfl_sync(0xffffffffu, x, boundary); };
+        merge = of(b_at, 0) < p.B && of(b_at, 0) == of(b_at, WARPS) && of(unit_at, 0) == of(unit_at, WARPS);
+        n = of(tiles_before, warp + 1) - of(tiles_before, warp);
+        if (tid == 0) {
+            sm.unit = unit_at;
+            sm.tile = tile_at;
         }
+        if (lane == 0) reinterpret_cast<Header *>(p.work)[me].last = -1;
+        at.b = of(b_at, warp);
+        at.len = of(len_at, warp);
+        at.tile = of(tile_at, warp);
+        at.tiles = tiles_of(at.len);
+        const int unit = of(unit_at, warp);
+        at.hk = (int)fdiv((uint32_t)unit, p.by_groups);
+        at.group = unit - at.hk * p.groups;
     }
     to = at;
     auto advance = [&](Cursor &c) {
@@ -520,13 +532,6 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attn_kernel(const __grid
     asm volatile("cp.async.wait_group 0;" ::: "memory");
 
     if (merge) {                // uniform over the CTA; the rings are done with
-        // the CTA's unit, which a warp without a tile knows from the schedule alone
-        int hk = at.hk, group = at.group;
-        if (!p.direct) {
-            hk = (int)fdiv((uint32_t)sm.at[0].unit, p.by_groups);
-            group = sm.at[0].unit - hk * p.groups;
-        }
-        const int rows = min(ROWS, p.G - group * ROWS), h0 = hk * p.G + group * ROWS;
         float *mine_o = reinterpret_cast<float *>(sm.ring[warp]), *mine_m = mine_o + ROWS * D;       // then the sums
         static_assert(sizeof(sm.ring[0]) >= part_floats(D) * sizeof(float), "a part in a warp's ring");
         __syncwarp();
@@ -545,7 +550,14 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attn_kernel(const __grid
             for (int j = 0; j < NT; ++j) *reinterpret_cast<float2 *>(mine_o + row * D + j * 8 + tq * 2) = make_float2(o[j][2 * r], o[j][2 * r + 1]);
         }
         __syncthreads();
-        float *part = p.direct ? nullptr : part_of(p, warps, D, blockIdx.x * WARPS, sm.at[0].tile == 0 ? 1 : 0);
+        // the CTA's unit, which a warp without a tile knows from the schedule alone
+        int hk = at.hk, group = at.group;
+        if (!p.direct) {
+            hk = (int)fdiv((uint32_t)sm.unit, p.by_groups);
+            group = sm.unit - hk * p.groups;
+        }
+        const int rows = min(ROWS, p.G - group * ROWS), h0 = hk * p.G + group * ROWS;
+        float *part = p.direct ? nullptr : part_of(p, warps, D, blockIdx.x * WARPS, sm.tile == 0 ? 1 : 0);
         for (int e = tid; e < rows * (D / 4); e += THREADS) {
             const int row = e / (D / 4), c = e % (D / 4) * 4;
             const float *from[WARPS];
