@@ -391,6 +391,18 @@ def test_prompt_then_tokens_equals_attention_over_the_whole(d, Hq, Hk, page):
     assert _lib.load().rgd_device_status() == 0
 
 
+@pytest.mark.parametrize("buckets,both,most", [(32, False, 5000), (512, True, 1000), (6, False, 200), (256, False, 129), (4, True, 1 << 20)])
+@pytest.mark.parametrize("wdtype", ["f32", "f16", "bf16"])
+def test_attention_bias_of_near_and_far_distances(buckets, both, most, wdtype):
+    """Borders on either side of where the kernel stops looking buckets up, for weights of every type."""
+    lengths = [4000, 255, 256, 257, 258, 1]
+    q, kc, vc, table, n = _case(lengths, 6, 3, 64, 16, "tokens", torch.bfloat16, buckets)
+    w = randn(gen(buckets), buckets, 6, dtype={"f32": torch.float32, **DTYPES}[wdtype])
+    o, lse = F_.paged_attention_func(q.cuda(), kc.cuda(), vc.cuda(), table.cuda(), n.cuda(), rel_weight=w.cuda(), bidirectional=both,
+                                     max_distance=most, return_lse=True)
+    P.assert_attention(o, lse, P.attention(q, kc, vc, table, n, 64 ** -0.5, w, both, most), "o")
+
+
 def test_position_bias_of_a_token_is_the_matrix_form_s_last_row():
     g = gen(14)
     m = ops.RelativePositionBias(32, 6, bidirectional=False).cuda()
