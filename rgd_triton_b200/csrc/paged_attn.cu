@@ -59,16 +59,18 @@ __device__ __forceinline__ int live_length(const AttnParams &p, int b, bool repo
 // this); with 16 keys of a tile each, added up at the unit's end, short sequences paid for that (103 us for 64 of 16
 // to 8192 keys, 72 like this).
 //
-// One B200, cold L2: 64 sequences of 16 to 8192 keys, 32 / 8 heads of 128 (366 MB) 72 us, one of 131 thousand (537 MB)
-// 97 us (104 on some of the GPUs).  Once the rings are full the keys arrive at 6.8 TB/s; 7 us go by before (lengths, table entries and first
-// tiles are reads that wait for one another), the warps end within 10 % of one another, and the join takes 3 us.
+// One B200, cold L2: 64 sequences of 16 to 8192 keys, 32 / 8 heads of 128 (366 MB) 70 us, one of 131 thousand (537 MB)
+// 92 us (100 on some of the GPUs).  6 us go by before the rings are full (lengths, table entries and first tiles are reads
+// that wait for one another), the warps end within 10 % of one another, and the join takes 3 us.  In between the two
+// warps of a scheduler are bound by the chain of a tile's instructions next to the reads: a tile without gaps is loaded
+// and scored without a check per key (long one 94.6 us with them).
 //
 // Weights are split into two numbers of the cache's type (hi + lo): rounded to one, they would cost as much accuracy
 // as the output's own rounding, and the matrix pipe idles anyway.
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int WARPS = 4, THREADS = WARPS * 32, ROWS = 16, STAGES = 3, CTAS_PER_SM = 2;
 // In tiles: what a unit's queries and output cost, and the least run of a warp.  us for 64 sequences of 16 to 8192 keys
-// with 8 cache heads / 48 of up to 2500 with 24: 71.6 / 35.8 like this, 72.2 / 36.9 at 2 and 3, 73.3 / 39.6 at 4 and 5.
+// with 8 cache heads / 48 of up to 2500 with 24: 70.5 / 34.4 like this, 70.9 / 35.7 at 2 and 3, 72.1 / 38.3 at 4 and 5.
 constexpr int UNIT_COST = 1, MIN_COST = 2;
 static_assert(MIN_COST > UNIT_COST, "a run that begins a unit has its first tile");
 
@@ -85,7 +87,10 @@ struct Smem {
         T k[KEYS * D], v[KEYS * D];
     };
     Stage ring[WARPS][STAGES];
-    int64_t row[WARPS][2][2 * KEYS];                    // of the tiles to load next: element offsets of keys, of values; -1: none
+    struct alignas(16) Row {
+        const T *k, *v;                                 // null: none
+    };
+    Row row[WARPS][2][KEYS];                            // of the tiles to load next
     int upto[THREADS], filled[THREADS];                 // costs and sequences with a token, of a warp's threads up to each
     int unit, tile;                                     // where the CTA's runs begin
     int borders[relbias::MAX_SIDE];                     // with a position bias
@@ -97,6 +102,9 @@ __device__ __forceinline__ void cp16(void *dst, const void *src, bool valid) {
     // not valid: nothing is read, 16 zero bytes are written
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src), "r"(valid ? 16 : 0)
                  : "memory");
+}
+__device__ __forceinline__ void cp16(void *dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
 }
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -298,30 +306,42 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attn_kernel(const __grid
     auto find = [&](const Fetched &f, int i) {
         const bool ok = f.slot >= 0 && page_ok(p.view, f.entry);
         if (f.slot >= 0 && !ok) g_attn_status = 1;
-        if (KEYS == 32 || lane < KEYS) sm.row[warp][i & 1][lane] = ok ? f.entry * p.k_sp + f.slot * p.k_ss + f.hk * p.k_sh : -1;
+        typename S::Row &row = sm.row[warp][i & 1][my_key];
+        if (KEYS == 32 || lane < KEYS)
+            row.k = ok ? reinterpret_cast<const T *>(p.k) + (f.entry * p.k_sp + f.slot * p.k_ss + f.hk * p.k_sh) : nullptr;
         if (KEYS == 32 || lane >= KEYS)
-            sm.row[warp][i & 1][KEYS + my_key] = ok ? f.entry * p.v_sp + f.slot * p.v_ss + f.hk * p.v_sh : -1;
+            row.v = ok ? reinterpret_cast<const T *>(p.v) + (f.entry * p.v_sp + f.slot * p.v_ss + f.hk * p.v_sh) : nullptr;
         return __ballot_sync(0xffffffffu, ok);
     };
-    auto load = [&](int i) {
+    constexpr uint32_t ALL = 0xffffffffu;       // the keys of a whole tile (those of 16 are there twice)
+    auto load = [&](int i, uint32_t there) {
         typename S::Stage &st = sm.ring[warp][i % STAGES];
         const int part = lane % CPR, c = part * 8;
-        const T *kg = reinterpret_cast<const T *>(p.k) + c, *vg = reinterpret_cast<const T *>(p.v) + c;
+        const typename S::Row *row = sm.row[warp][i & 1] + lane / CPR;
+        auto to = [&](int j) { return (j * RPP + lane / CPR) * D + (part ^ ((j * RPP + lane / CPR) & 7)) * 8; };
+        if (VEC && there == ALL && p.d == D) {
+#pragma unroll
+            for (int j = 0; j < PASSES; ++j) {
+                const typename S::Row from = row[j * RPP];
+                cp16(st.k + to(j), from.k + c);
+                cp16(st.v + to(j), from.v + c);
+            }
+            return;
+        }
 #pragma unroll
         for (int j = 0; j < PASSES; ++j) {
-            const int r = j * RPP + lane / CPR, to_c = r * D + (part ^ (r & 7)) * 8;
-            const int64_t kr = sm.row[warp][i & 1][r], vr = sm.row[warp][i & 1][KEYS + r];
-            T *kd = st.k + to_c, *vd = st.v + to_c;
+            const typename S::Row from = row[j * RPP];
+            T *kd = st.k + to(j), *vd = st.v + to(j);
             if constexpr (VEC) {
-                const bool in = kr >= 0 && c < p.d;
-                cp16(kd, in ? kg + kr : p.k, in);
-                cp16(vd, in ? vg + vr : p.v, in);
+                const bool in = from.k && c < p.d;
+                cp16(kd, in ? from.k + c : p.k, in);
+                cp16(vd, in ? from.v + c : p.v, in);
             } else {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const bool in = kr >= 0 && c + e < p.d;
-                    kd[e] = in ? kg[kr + e] : from_f32<T>(0.f);
-                    vd[e] = in ? vg[vr + e] : from_f32<T>(0.f);
+                    const bool in = from.k && c + e < p.d;
+                    kd[e] = in ? from.k[c + e] : from_f32<T>(0.f);
+                    vd[e] = in ? from.v[c + e] : from_f32<T>(0.f);
                 }
             }
         }
@@ -369,7 +389,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attn_kernel(const __grid
             if (i < n) {
                 live[i] = find(f[i], i);
                 __syncwarp();
-                if (i < STAGES - 1) load(i);
+                if (i < STAGES - 1) load(i, live[i]);
                 __syncwarp();           // the third tile's rows go where the first one's were
             }
             if (i < STAGES - 1) asm volatile("cp.async.commit_group;" ::: "memory");
@@ -413,7 +433,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attn_kernel(const __grid
         }
         asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
         __syncwarp();                   // this tile has landed; all lanes are done with the tile before it
-        if (i + STAGES - 1 < n) load(i + STAGES - 1);
+        if (i + STAGES - 1 < n) load(i + STAGES - 1, live[STAGES - 1]);
         asm volatile("cp.async.commit_group;" ::: "memory");
         if (i + STAGES < n) {
             live[STAGES] = find(next, i + STAGES);
@@ -443,21 +463,24 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attn_kernel(const __grid
                     for (int e = 0; e < 4; ++e)
                         add[t][e] = p.w_dtype == RGD_BF16 ? add[t][e] << 16 : __float_as_uint(__half2float(__ushort_as_half((uint16_t)add[t][e])));
         }
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                s[t][e] *= p.scale_log2;
+                if constexpr (BIAS) s[t][e] += attn::bias_log2<float>(__uint_as_float(add[t][e]));
+            }
+        if (live[0] != ALL)
+#pragma unroll
+            for (int t = 0; t < KT; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (!(live[0] >> (t * 8 + tq * 2 + (e & 1)) & 1)) s[t][e] = -INFINITY;
         float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
         for (int t = 0; t < KT; ++t)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int key = t * 8 + tq * 2 + e;
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    float x = s[t][r * 2 + e] * p.scale_log2;
-                    if constexpr (BIAS) x += attn::bias_log2<float>(__uint_as_float(add[t][r * 2 + e]));
-                    if (!(live[0] >> key & 1)) x = -INFINITY;
-                    s[t][r * 2 + e] = x;
-                    mx[r] = fmaxf(mx[r], x);
-                }
-            }
+            for (int e = 0; e < 4; ++e) mx[e >> 1] = fmaxf(mx[e >> 1], s[t][e]);
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
             mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
@@ -759,10 +782,11 @@ bool too_large(int64_t B, int64_t units, int64_t max_keys, int D) {
 // How the tiles are spread.  Few units of few keys (by what the table has room for; the lengths are not known here): a CTA
 // per unit, which needs no schedule, no workspace and no second launch.  Others: what the SMs hold at once, and no more
 // CTAs than there can be runs.  us of GPU time in equal runs / a CTA per unit, at 8, 16, 24, 32, 48 tiles:
-//   16 units, head_dim 128    16.4 / 10.2   16.4 / 14.3   18.4 / 16.4   18.4 / 18.4   18.4 / 24.6
-//   256 units, head_dim 64    18.4 / 12.3   20.5 / 16.4   24.6 / 20.5   26.6 / 24.6   32.8 / 30.7
-//   512 units, head_dim 128   22.5 / 20.5   26.6 / 26.6   34.8 / 34.8   41.0 / 41.0   51.2 / 53.2
-//   2048 units, head_dim 128  41.0 / 53.2   63.5 / 75.8   84.0 / 102    107 / 125     147 / 168
+//   16 units, head_dim 64     14.3 / 8.2    14.3 / 12.3   14.3 / 14.3   14.3 / 18.4   14.3 / 22.5
+//   64 units, head_dim 128    14.3 / 10.2   14.3 / 12.3   16.4 / 16.4   16.4 / 18.4   18.4 / 24.6
+//   256 units, head_dim 64    16.4 / 12.3   18.4 / 14.4   20.5 / 18.4   24.6 / 22.5   30.7 / 28.7
+//   512 units, head_dim 128   18.4 / 18.4   24.5 / 24.6   30.7 / 32.8   36.9 / 38.9   47.1 / 51.2
+//   2048 units, head_dim 128  36.8 / 51.2   59.4 / 73.7   81.9 / 100    102 / 121     143 / 164
 constexpr int DIRECT_TILES = 28;
 struct Plan {
     bool direct;
