@@ -151,11 +151,19 @@ struct Cursor {
     int b, hk, group, tile, tiles, len;
 };
 
-template <typename T, int D, bool VEC, bool BIAS>
+// The transpose of an 8 x 8 matrix of 16-bit elements in a warp's registers.
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+// HT: column tiles of 8 query heads.
+template <typename T, int D, bool VEC, bool BIAS, int HT>
 __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attn_kernel(const __grid_constant__ AttnParams p) {
     using S = Smem<T, D>;
     constexpr int KEYS = S::KEYS, CPR = D / 8, RPP = 32 / CPR, PASSES = KEYS / RPP;      // 16-byte chunks of a row, rows a warp copies at once
-    constexpr int NT = D / 8, KT = KEYS / 8;                // column tiles of the output, of the scores
+    constexpr int MT = D / 16, KT = KEYS / 16;              // row tiles of the output, of the scores
     extern __shared__ __align__(16) unsigned char raw[];
     S &sm = *reinterpret_cast<S *>(raw);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gq = lane >> 2, tq = lane & 3;
@@ -346,13 +354,23 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attn_kernel(const __grid
             }
         }
     };
-    uint32_t aq[D / 16][4];             // the unit's queries as A fragments, rows past the group and channels past d as zeros
-    float o[NT][4];                     // rows gq and gq + 8
+    // Keys are the rows of the scores and channels the rows of the output, heads the columns of both: few heads leave no
+    // rows empty.  A lane has the heads 8 h + 2 tq and the next one.
+    uint32_t bq[D / 16][HT][2];         // the unit's queries as B fragments, heads past the group and channels past d as zeros
+    float o[MT][HT][4];
+    float m_ref[HT][2], l_sum[HT][2];
+    auto clear = [&]() {
 #pragma unroll
-    for (int j = 0; j < NT; ++j)
+        for (int h = 0; h < HT; ++h) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[j][e] = 0.f;          // a warp without a tile has its part in a unit's end too
-    float m_ref[2] = {-INFINITY, -INFINITY}, l_sum[2] = {0.f, 0.f};
+            for (int j = 0; j < MT; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[j][h][e] = 0.f;
+            m_ref[h][0] = m_ref[h][1] = -INFINITY;
+            l_sum[h][0] = l_sum[h][1] = 0.f;
+        }
+    };
+    clear();                            // a warp without a tile has its part in a unit's end too
     bool whole = false;                 // the unit's first tile was in this run
     const int mi = lane >> 3, mr = lane & 7;
 
@@ -362,16 +380,45 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attn_kernel(const __grid
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int r = gq + (e & 1) * 8, c = kk * 16 + (e >> 1) * 8 + tq * 2;
-                uint32_t x = 0u;
-                if constexpr (VEC) {
-                    if (r < rows && c < p.d) x = *reinterpret_cast<const uint32_t *>(qg + (int64_t)r * p.q_sh + c);
-                } else if (r < rows) {
-                    const T *qr = qg + (int64_t)r * p.q_sh + c;
-                    x = attn::Mma<T>::pack(c < p.d ? to_f32<T>(qr[0]) : 0.f, c + 1 < p.d ? to_f32<T>(qr[1]) : 0.f);
+            for (int h = 0; h < HT; ++h)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int r = h * 8 + gq, c = kk * 16 + e * 8 + tq * 2;
+                    uint32_t x = 0u;
+                    if constexpr (VEC) {
+                        if (r < rows && c < p.d) x = *reinterpret_cast<const uint32_t *>(qg + (int64_t)r * p.q_sh + c);
+                    } else if (r < rows) {
+                        const T *qr = qg + (int64_t)r * p.q_sh + c;
+                        x = attn::Mma<T>::pack(c < p.d ? to_f32<T>(qr[0]) : 0.f, c + 1 < p.d ? to_f32<T>(qr[1]) : 0.f);
+                    }
+                    bq[kk][h][e] = x;
                 }
-                aq[kk][e] = x;
+    };
+
+    // A unit's end: the lanes' sums are added up, its numbers written as a part.
+    auto add_lanes = [&]() {
+#pragma unroll
+        for (int h = 0; h < HT; ++h)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int x = 4; x < 32; x *= 2) l_sum[h][e] += __shfl_xor_sync(0xffffffffu, l_sum[h][e], x);
+    };
+    auto store_part = [&](float *to_o, float *to_m, int rows) {
+#pragma unroll
+        for (int h = 0; h < HT; ++h)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int row = h * 8 + tq * 2 + e;
+                if (row >= rows) continue;
+                if (gq == 0) {
+                    to_m[row] = m_ref[h][e];
+                    to_m[ROWS + row] = l_sum[h][e];
+                }
+#pragma unroll
+                for (int j = 0; j < MT; ++j)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) to_o[row * D + j * 16 + r * 8 + gq] = o[j][h][r * 2 + e];
             }
     };
 
@@ -402,18 +449,15 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attn_kernel(const __grid
         const int h0 = at.hk * p.G + row0;              // query head of row 0
         if (i == 0 || at.tile == 0) {
             whole = at.tile == 0;
-            if (i > 0) read_queries();
-#pragma unroll
-            for (int j = 0; j < NT; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[j][e] = 0.f;
-            m_ref[0] = m_ref[1] = -INFINITY;
-            l_sum[0] = l_sum[1] = 0.f;
+            if (i > 0) {
+                read_queries();
+                clear();
+            }
         }
         // The position bias, read while the tile is on its way and converted when it is used: a conversion behind each
         // read would make the reads wait for one another (17.3 us for 16 sequences of up to 1500 tokens, 16.3 like this;
         // 15.1 with the buckets of near distances looked up instead of searched).
-        uint32_t add[BIAS ? KT : 1][4];
+        uint32_t add[BIAS ? KT : 1][HT][4];
         if constexpr (BIAS) {
             const int far = max(at.len - 1 - (at.tile * KEYS + my_key), 0);
             const int bucket = far < NEAR ? sm.bucket[far] : far >= last_border ? p.borders.side - 1
@@ -422,10 +466,13 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attn_kernel(const __grid
 #pragma unroll
                 for (int t = 0; t < KT; ++t)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int64_t w_at = __shfl_sync(0xffffffffu, bucket, t * 8 + tq * 2 + e) * p.w_sk + (h0 + gq) * p.w_sh;
+                    for (int r = 0; r < 2; ++r) {
+                        const int64_t w_at = __shfl_sync(0xffffffffu, bucket, t * 16 + r * 8 + gq) * p.w_sk + (h0 + tq * 2) * p.w_sh;
 #pragma unroll
-                        for (int r = 0; r < 2; ++r) add[t][r * 2 + e] = gq + r * 8 < rows ? w[w_at + r * 8 * p.w_sh] : 0u;
+                        for (int h = 0; h < HT; ++h)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e)
+                                add[t][h][r * 2 + e] = h * 8 + tq * 2 + e < rows ? w[w_at + (h * 8 + e) * p.w_sh] : 0u;
                     }
             };
             if (p.w_dtype == RGD_F32) read_bias(reinterpret_cast<const uint32_t *>(p.w));
@@ -441,89 +488,106 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attn_kernel(const __grid
         }
         const typename S::Stage &st = sm.ring[warp][i % STAGES];
 
-        float s[KT][4];
+        float s[KT][HT][4], s2[KT][HT][4];      // two sums, of every other 16 channels: shorter chains
 #pragma unroll
         for (int t = 0; t < KT; ++t)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[t][e] = 0.f;
+            for (int h = 0; h < HT; ++h)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[t][h][e] = s2[t][h][e] = 0.f;
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk)
 #pragma unroll
-            for (int t = 0; t < KT; t += 2) {
-                uint32_t bf[4];
-                attn::ldmatrix_x4(bf, st.k + (t * 8 + mr + (mi >> 1) * 8) * D + ((kk * 2 + (mi & 1)) ^ mr) * 8);
-                attn::Mma<T>::mma(s[t], aq[kk], bf[0], bf[1]);
-                attn::Mma<T>::mma(s[t + 1], aq[kk], bf[2], bf[3]);
+            for (int t = 0; t < KT; ++t) {
+                uint32_t a[4];
+                attn::ldmatrix_x4(a, st.k + (t * 16 + (mi & 1) * 8 + mr) * D + ((kk * 2 + (mi >> 1)) ^ mr) * 8);
+#pragma unroll
+                for (int h = 0; h < HT; ++h) attn::Mma<T>::mma(kk % 2 ? s2[t][h] : s[t][h], a, bq[kk][h][0], bq[kk][h][1]);
             }
         if constexpr (BIAS) {
             if (p.w_dtype != RGD_F32)
 #pragma unroll
                 for (int t = 0; t < KT; ++t)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        add[t][e] = p.w_dtype == RGD_BF16 ? add[t][e] << 16 : __float_as_uint(__half2float(__ushort_as_half((uint16_t)add[t][e])));
+                    for (int h = 0; h < HT; ++h)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            add[t][h][e] = p.w_dtype == RGD_BF16 ? add[t][h][e] << 16
+                                                                 : __float_as_uint(__half2float(__ushort_as_half((uint16_t)add[t][h][e])));
         }
 #pragma unroll
         for (int t = 0; t < KT; ++t)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                s[t][e] *= p.scale_log2;
-                if constexpr (BIAS) s[t][e] += attn::bias_log2<float>(__uint_as_float(add[t][e]));
-            }
+            for (int h = 0; h < HT; ++h)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    s[t][h][e] = (s[t][h][e] + s2[t][h][e]) * p.scale_log2;
+                    if constexpr (BIAS) s[t][h][e] += attn::bias_log2<float>(__uint_as_float(add[t][h][e]));
+                }
         if (live[0] != ALL)
 #pragma unroll
             for (int t = 0; t < KT; ++t)
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    if (!(live[0] >> (t * 8 + tq * 2 + (e & 1)) & 1)) s[t][e] = -INFINITY;
-        float mx[2] = {-INFINITY, -INFINITY};
+                    if (!(live[0] >> (t * 16 + (e >> 1) * 8 + gq) & 1))
 #pragma unroll
-        for (int t = 0; t < KT; ++t)
+                        for (int h = 0; h < HT; ++h) s[t][h][e] = -INFINITY;
+        float mx[HT][2];
+        bool more = false;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) mx[e >> 1] = fmaxf(mx[e >> 1], s[t][e]);
+        for (int h = 0; h < HT; ++h)
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
-            mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
-        }
+            for (int e = 0; e < 2; ++e) {
+                mx[h][e] = fmaxf(s[0][h][e], s[0][h][2 + e]);
+#pragma unroll
+                for (int t = 1; t < KT; ++t) mx[h][e] = fmaxf(mx[h][e], fmaxf(s[t][h][e], s[t][h][2 + e]));
+                more |= mx[h][e] > m_ref[h][e];
+            }
         // the reference follows the maximum: a new one gets rare along the keys
-        const bool more[2] = {mx[0] > m_ref[0], mx[1] > m_ref[1]};
-        if (__any_sync(0xffffffffu, more[0] || more[1])) {
+        if (__any_sync(0xffffffffu, more)) {
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const float alpha = !more[r] ? 1.f : m_ref[r] == -INFINITY ? 0.f : ex2(m_ref[r] - mx[r]);
-                if (more[r]) m_ref[r] = mx[r];
-                l_sum[r] *= alpha;
+            for (int h = 0; h < HT; ++h)
 #pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    o[j][2 * r] *= alpha;
-                    o[j][2 * r + 1] *= alpha;
+                for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                    for (int x = 4; x < 32; x *= 2) mx[h][e] = fmaxf(mx[h][e], __shfl_xor_sync(0xffffffffu, mx[h][e], x));
+                    if (!(mx[h][e] > m_ref[h][e])) continue;
+                    const float alpha = m_ref[h][e] == -INFINITY ? 0.f : ex2(m_ref[h][e] - mx[h][e]);
+                    m_ref[h][e] = mx[h][e];
+                    l_sum[h][e] *= alpha;
+#pragma unroll
+                    for (int j = 0; j < MT; ++j) {
+                        o[j][h][e] *= alpha;
+                        o[j][h][2 + e] *= alpha;
+                    }
                 }
-            }
         }
 #pragma unroll
-        for (int kk = 0; kk < KT / 2; ++kk) {
-            uint32_t hi[4], lo[4];
+        for (int t = 0; t < KT; ++t) {
+            uint32_t hi[HT][2], lo[HT][2];
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const float mu = m_ref[r] == -INFINITY ? 0.f : m_ref[r];
+            for (int h = 0; h < HT; ++h)
 #pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    const float p0 = ex2(s[2 * kk + t][2 * r] - mu), p1 = ex2(s[2 * kk + t][2 * r + 1] - mu);
-                    l_sum[r] += p0 + p1;
-                    const float r0 = round_to<T>(p0), r1 = round_to<T>(p1);
-                    hi[t * 2 + r] = attn::Mma<T>::pack(r0, r1);
-                    lo[t * 2 + r] = attn::Mma<T>::pack(p0 - r0, p1 - r1);
+                for (int r = 0; r < 2; ++r) {
+                    float pr[2], rest[2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        pr[e] = ex2(s[t][h][r * 2 + e] - (m_ref[h][e] == -INFINITY ? 0.f : m_ref[h][e]));
+                        l_sum[h][e] += pr[e];
+                        rest[e] = pr[e] - round_to<T>(pr[e]);
+                    }
+                    hi[h][r] = transposed(attn::Mma<T>::pack(pr[0], pr[1]));
+                    lo[h][r] = transposed(attn::Mma<T>::pack(rest[0], rest[1]));
                 }
-            }
 #pragma unroll
-            for (int j = 0; j < NT; j += 2) {
-                uint32_t bf[4];
-                attn::ldmatrix_x4_trans(bf, st.v + (kk * 16 + mr + (mi & 1) * 8) * D + ((j + (mi >> 1)) ^ mr) * 8);
-                attn::Mma<T>::mma(o[j], hi, bf[0], bf[1]);
-                attn::Mma<T>::mma(o[j + 1], hi, bf[2], bf[3]);
-                attn::Mma<T>::mma(o[j], lo, bf[0], bf[1]);
-                attn::Mma<T>::mma(o[j + 1], lo, bf[2], bf[3]);
+            for (int j = 0; j < MT; ++j) {
+                uint32_t a[4];
+                attn::ldmatrix_x4_trans(a, st.v + (t * 16 + (mi >> 1) * 8 + mr) * D + ((j * 2 + (mi & 1)) ^ mr) * 8);
+#pragma unroll
+                for (int h = 0; h < HT; ++h) {
+                    attn::Mma<T>::mma(o[j][h], a, hi[h][0], hi[h][1]);
+                    attn::Mma<T>::mma(o[j][h], a, lo[h][0], lo[h][1]);
+                }
             }
         }
 #pragma unroll
@@ -531,37 +595,39 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attn_kernel(const __grid
 
         const bool done = at.tile == at.tiles - 1;
         if (!p.direct && (done || i == n - 1)) {
+            add_lanes();
+            if (done && whole) {
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                l_sum[r] += __shfl_xor_sync(0xffffffffu, l_sum[r], 1);
-                l_sum[r] += __shfl_xor_sync(0xffffffffu, l_sum[r], 2);
-                const int row = gq + r * 8;
-                if (row >= rows) continue;
-                if (done && whole) {
-                    const float inv = l_sum[r] == 0.f ? 0.f : 1.f / l_sum[r];
-                    T *out = reinterpret_cast<T *>(p.o) + (int64_t)at.b * p.o_sb + (int64_t)(h0 + row) * p.o_sh;
+                for (int h = 0; h < HT; ++h) {
+                    float inv[2];
 #pragma unroll
-                    for (int j = 0; j < NT; ++j) {
-                        const int c = j * 8 + tq * 2;
-                        if constexpr (VEC) {
-                            if (c < p.d) *reinterpret_cast<uint32_t *>(out + c) = attn::Mma<T>::pack(o[j][2 * r] * inv, o[j][2 * r + 1] * inv);
-                        } else {
-                            if (c < p.d) out[c] = from_f32<T>(o[j][2 * r] * inv);
-                            if (c + 1 < p.d) out[c + 1] = from_f32<T>(o[j][2 * r + 1] * inv);
+                    for (int e = 0; e < 2; ++e) {
+                        const int row = h * 8 + tq * 2 + e;
+                        inv[e] = l_sum[h][e] == 0.f ? 0.f : 1.f / l_sum[h][e];
+                        if (p.lse && gq == 0 && row < rows)
+                            p.lse[(int64_t)at.b * p.Hq + h0 + row] = l_sum[h][e] == 0.f ? -INFINITY : (m_ref[h][e] + log2f(l_sum[h][e])) * LN2;
+                    }
+                    T *out = reinterpret_cast<T *>(p.o) + (int64_t)at.b * p.o_sb + (int64_t)(h0 + h * 8 + gq) * p.o_sh;
+#pragma unroll
+                    for (int j = 0; j < MT; ++j)
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) {
+                            // a head's two neighbouring channels, for one store
+                            const uint32_t y = transposed(attn::Mma<T>::pack(o[j][h][r * 2] * inv[0], o[j][h][r * 2 + 1] * inv[1]));
+                            const int c = j * 16 + r * 8 + tq * 2;
+                            if (h * 8 + gq >= rows) continue;
+                            if constexpr (VEC) {
+                                if (c < p.d) *reinterpret_cast<uint32_t *>(out + c) = y;
+                            } else {
+                                const uint16_t y0 = (uint16_t)y, y1 = (uint16_t)(y >> 16);
+                                if (c < p.d) reinterpret_cast<uint16_t *>(out)[c] = y0;
+                                if (c + 1 < p.d) reinterpret_cast<uint16_t *>(out)[c + 1] = y1;
+                            }
                         }
-                    }
-                    if (p.lse && tq == 0)
-                        p.lse[(int64_t)at.b * p.Hq + h0 + row] = l_sum[r] == 0.f ? -INFINITY : (m_ref[r] + log2f(l_sum[r])) * LN2;
-                } else if (!merge) {
-                    float *part = part_of(p, warps, D, me, whole ? 1 : 0);
-                    if (tq == 0) {
-                        part[row] = m_ref[r];
-                        part[ROWS + row] = l_sum[r];
-                    }
-#pragma unroll
-                    for (int j = 0; j < NT; ++j)
-                        *reinterpret_cast<float2 *>(part + 2 * ROWS + row * D + j * 8 + tq * 2) = make_float2(o[j][2 * r], o[j][2 * r + 1]);
                 }
+            } else if (!merge) {
+                float *part = part_of(p, warps, D, me, whole ? 1 : 0);
+                store_part(part + 2 * ROWS, part, rows);
             }
             if (!done && whole && lane == 0) {
                 // this run ends before the tiles that are left of the unit
@@ -580,21 +646,9 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attn_kernel(const __grid
     if (merge) {                // uniform over the CTA; the rings are done with
         float *mine_o = reinterpret_cast<float *>(sm.ring[warp]), *mine_m = mine_o + ROWS * D;       // then the sums
         static_assert(sizeof(sm.ring[0]) >= part_floats(D) * sizeof(float), "a part in a warp's ring");
+        if (p.direct) add_lanes();      // a run's end has done it otherwise
         __syncwarp();
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const int row = gq + r * 8;
-            if (p.direct) {             // a run's end has done it otherwise
-                l_sum[r] += __shfl_xor_sync(0xffffffffu, l_sum[r], 1);
-                l_sum[r] += __shfl_xor_sync(0xffffffffu, l_sum[r], 2);
-            }
-            if (tq == 0) {
-                mine_m[row] = m_ref[r];
-                mine_m[ROWS + row] = l_sum[r];
-            }
-#pragma unroll
-            for (int j = 0; j < NT; ++j) *reinterpret_cast<float2 *>(mine_o + row * D + j * 8 + tq * 2) = make_float2(o[j][2 * r], o[j][2 * r + 1]);
-        }
+        store_part(mine_o, mine_m, ROWS);
         __syncthreads();
         // the CTA's unit, which a warp without a tile knows from the schedule alone
         int hk = at.hk, group = at.group;
@@ -802,7 +856,7 @@ Plan make_plan(int64_t B, int64_t units, int64_t max_keys, int D) {
 
 template <typename T, int D, bool VEC, bool BIAS>
 int launch(AttnParams &p, const Plan &plan, cudaStream_t st) {
-    auto kernel = attn_kernel<T, D, VEC, BIAS>;
+    auto kernel = p.G <= 8 ? attn_kernel<T, D, VEC, BIAS, 1> : attn_kernel<T, D, VEC, BIAS, 2>;
     constexpr size_t smem = sizeof(Smem<T, D>);
     static_assert(CTAS_PER_SM * (smem + 1024) <= 228 << 10, "shared memory of an SM");
     if (int e = ensure_dyn_smem(reinterpret_cast<const void *>(kernel), smem)) return e;
