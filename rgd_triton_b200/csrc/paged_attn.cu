@@ -46,7 +46,7 @@ __device__ __forceinline__ int live_length(const AttnParams &p, int b, bool repo
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// Work.  A unit is a sequence, a cache head and up to 16 of the query heads that share it (one m16n8k16 row tile);
+// Work.  A unit is a sequence, a cache head and up to 16 of the query heads that share it (one or two column tiles of 8);
 // its keys come in tiles.  The tiles of all units, one after the other, are dealt out to the warps of the grid in runs
 // of equal cost, whatever the lengths are; a CTA finds its warps' runs from the lengths, which are on the device.  A unit
 // that one warp has whole is finished there; of a unit that several have, each leaves its part (row maximum, row sum,
@@ -55,28 +55,32 @@ __device__ __forceinline__ int live_length(const AttnParams &p, int b, bool repo
 // A warp does everything for its tiles: it streams the keys and values through a ring of cp.async stages of its own,
 // which goes on across units, keeps the running maximum, sum and output in registers, and waits for no other warp.
 // Two forms in which the four warps of a CTA shared a unit were slower: with the maxima and weights of a tile exchanged
-// and the channels split, three barriers a tile held the loop (120 us for one sequence of 131 thousand keys, 93 us like
-// this); with 16 keys of a tile each, added up at the unit's end, short sequences paid for that (103 us for 64 of 16
-// to 8192 keys, 72 like this).
+// and the channels split, three barriers a tile held the loop (120 us for one sequence of 131 thousand keys, 93 us
+// without); with 16 keys of a tile each, added up at the unit's end, short sequences paid for that (103 us for 64 of 16
+// to 8192 keys, 72 us without).
 //
-// One B200, cold L2: 64 sequences of 16 to 8192 keys, 32 / 8 heads of 128 (366 MB) 70 us, one of 131 thousand (537 MB)
-// 92 us (100 on some of the GPUs).  6 us go by before the rings are full (lengths, table entries and first tiles are reads
-// that wait for one another), the warps end within 10 % of one another, and the join takes 3 us.  In between the two
-// warps of a scheduler are bound by the chain of a tile's instructions next to the reads: a tile without gaps is loaded
-// and scored without a check per key (long one 94.6 us with them).
+// One B200, cold L2: 64 sequences of 16 to 8192 keys, 32 / 8 heads of 128 (366 MB) 65 us, one of 131 thousand (537 MB)
+// 90 us (98 on some of the GPUs).  6 us go by before the rings are full (lengths, table entries and first tiles are reads
+// that wait for one another) and the join takes 3-4 us; in between the keys arrive at the copy rate.
+//
+// With two warps on a scheduler the chain of a tile's instructions counts next to the reads.  So a tile without gaps is
+// loaded and scored without a check per key (95 us for the long one with them), and the products are taken transposed:
+// up to eight query heads of a cache head are one column tile, where as rows they would leave half of a row tile's
+// scores, weights and sums empty (70 us for the 64, 9.8 instead of 8.5 for one sequence of 300).
 //
 // Weights are split into two numbers of the cache's type (hi + lo): rounded to one, they would cost as much accuracy
 // as the output's own rounding, and the matrix pipe idles anyway.
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int WARPS = 4, THREADS = WARPS * 32, ROWS = 16, STAGES = 3, CTAS_PER_SM = 2;
 // In tiles: what a unit's queries and output cost, and the least run of a warp.  us for 64 sequences of 16 to 8192 keys
-// with 8 cache heads / 48 of up to 2500 with 24: 70.5 / 34.4 like this, 70.9 / 35.7 at 2 and 3, 72.1 / 38.3 at 4 and 5.
-constexpr int UNIT_COST = 1, MIN_COST = 2;
+// with 8 cache heads / 48 of up to 2500 with 24 / 16 of up to 1500 with 16: 65.3 / 32.3 / 13.4 like this, 65.4 / 32.0 / 13.8
+// at 1 and 2, 65.7 / 32.8 / 13.3 at 3 and 4.
+constexpr int UNIT_COST = 2, MIN_COST = 3;
 static_assert(MIN_COST > UNIT_COST, "a run that begins a unit has its first tile");
 
 __host__ __device__ constexpr int tile_keys(int D) { return D > 64 ? 16 : 32; }      // 8 KB of keys and values
 
-constexpr int NEAR = 256;
+constexpr int NEAR = 256;               // distances whose bucket is looked up
 
 template <typename T, int D>
 struct Smem {
@@ -455,8 +459,8 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attn_kernel(const __grid
             }
         }
         // The position bias, read while the tile is on its way and converted when it is used: a conversion behind each
-        // read would make the reads wait for one another (17.3 us for 16 sequences of up to 1500 tokens, 16.3 like this;
-        // 15.1 with the buckets of near distances looked up instead of searched).
+        // read would make the reads wait for one another (1.0 us of 16 sequences of up to 1500 tokens; the buckets of
+        // near distances are looked up, to search for them would cost 1.2 us).
         uint32_t add[BIAS ? KT : 1][HT][4];
         if constexpr (BIAS) {
             const int far = max(at.len - 1 - (at.tile * KEYS + my_key), 0);
@@ -836,11 +840,11 @@ bool too_large(int64_t B, int64_t units, int64_t max_keys, int D) {
 // How the tiles are spread.  Few units of few keys (by what the table has room for; the lengths are not known here): a CTA
 // per unit, which needs no schedule, no workspace and no second launch.  Others: what the SMs hold at once, and no more
 // CTAs than there can be runs.  us of GPU time in equal runs / a CTA per unit, at 8, 16, 24, 32, 48 tiles:
-//   16 units, head_dim 64     14.3 / 8.2    14.3 / 12.3   14.3 / 14.3   14.3 / 18.4   14.3 / 22.5
-//   64 units, head_dim 128    14.3 / 10.2   14.3 / 12.3   16.4 / 16.4   16.4 / 18.4   18.4 / 24.6
-//   256 units, head_dim 64    16.4 / 12.3   18.4 / 14.4   20.5 / 18.4   24.6 / 22.5   30.7 / 28.7
-//   512 units, head_dim 128   18.4 / 18.4   24.5 / 24.6   30.7 / 32.8   36.9 / 38.9   47.1 / 51.2
-//   2048 units, head_dim 128  36.8 / 51.2   59.4 / 73.7   81.9 / 100    102 / 121     143 / 164
+//   16 units, head_dim 64     14.3 / 10.2   14.3 / 12.3   14.3 / 14.3   14.3 / 16.5   14.3 / 22.5
+//   64 units, head_dim 128    14.3 / 10.2   14.3 / 12.3   16.4 / 14.3   16.4 / 18.4   18.4 / 22.5
+//   256 units, head_dim 64    16.4 / 12.3   18.4 / 14.3   22.5 / 18.4   24.6 / 20.5   28.7 / 26.6
+//   512 units, head_dim 128   20.5 / 18.4   24.6 / 24.6   28.7 / 28.7   34.8 / 34.8   44.9 / 45.1
+//   2048 units, head_dim 128  36.9 / 45.1   57.3 / 67.6   77.8 / 90.1   98.3 / 109    139 / 143
 constexpr int DIRECT_TILES = 28;
 struct Plan {
     bool direct;
