@@ -60,7 +60,7 @@ __device__ __forceinline__ int live_length(const AttnParams &p, int b, bool repo
 // to 8192 keys, 72 us without).
 //
 // One B200, cold L2: 64 sequences of 16 to 8192 keys, 32 / 8 heads of 128 (366 MB) 65 us, one of 131 thousand (537 MB)
-// 90 us (98 on some of the GPUs).  6 us go by before the rings are full (lengths, table entries and first tiles are reads
+// 90 us (some GPUs take 7 % longer).  6 us go by before the rings are full (lengths, table entries and first tiles are reads
 // that wait for one another) and the join takes 3-4 us; in between the keys arrive at the copy rate.
 //
 // With two warps on a scheduler the chain of a tile's instructions counts next to the reads.  So a tile without gaps is
