@@ -391,6 +391,22 @@ def test_prompt_then_tokens_equals_attention_over_the_whole(d, Hq, Hk, page):
     assert _lib.load().rgd_device_status() == 0
 
 
+@pytest.mark.parametrize("G", [1, 2, 7, 8, 9, 15, 16, 17, 24, 25, 33])
+@pytest.mark.parametrize("d,page", [(64, 16), (128, 24), (100, 16)])
+def test_attention_of_any_number_of_heads_to_a_cache_head(G, d, page):
+    """One and two column tiles of heads, whole and not, groups of 16; with and without a schedule; twice the same bits."""
+    for lengths in ([300, 1, 77], [3000, 20, 500]):
+        q, kc, vc, table, n = _case(lengths, 2 * G, 2, d, page, "tokens", torch.bfloat16, G + d)
+        w = randn(gen(G), 32, 2 * G)
+        for bias in (None, w):
+            args = {} if bias is None else {"rel_weight": bias.cuda()}
+            call = lambda: F_.paged_attention_func(q.cuda(), kc.cuda(), vc.cuda(), table.cuda(), n.cuda(), return_lse=True, **args)
+            o, lse = call()
+            P.assert_attention(o, lse, P.attention(q, kc, vc, table, n, d ** -0.5, bias, *(() if bias is None else (False, 128))), (lengths, G))
+            again = call()
+            assert torch.equal(o, again[0]) and torch.equal(lse, again[1])
+
+
 @pytest.mark.parametrize("buckets,both,most", [(32, False, 5000), (512, True, 1000), (6, False, 200), (256, False, 129), (4, True, 1 << 20)])
 @pytest.mark.parametrize("wdtype", ["f32", "f16", "bf16"])
 def test_attention_bias_of_near_and_far_distances(buckets, both, most, wdtype):
