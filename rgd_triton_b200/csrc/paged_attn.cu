@@ -27,7 +27,7 @@ struct AttnParams {
     int64_t o_sb, o_sh;
     float *lse;                             // null: not wanted
     int B, Hq, Hkv, G, d;                   // G: query heads of a cache head
-    int groups, units;                      // row tiles of a cache head, of a sequence
+    int groups, units;                      // units of a cache head, of a sequence
     FastDiv by_units, by_groups;
     int direct;                             // a CTA per unit, nothing to join
     char *work;
@@ -556,9 +556,9 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attn_kernel(const __grid
                 for (int e = 0; e < 2; ++e) {
 #pragma unroll
                     for (int x = 4; x < 32; x *= 2) mx[h][e] = fmaxf(mx[h][e], __shfl_xor_sync(0xffffffffu, mx[h][e], x));
-                    if (!(mx[h][e] > m_ref[h][e])) continue;
-                    const float alpha = m_ref[h][e] == -INFINITY ? 0.f : ex2(m_ref[h][e] - mx[h][e]);
-                    m_ref[h][e] = mx[h][e];
+                    const bool higher = mx[h][e] > m_ref[h][e];
+                    const float alpha = !higher ? 1.f : m_ref[h][e] == -INFINITY ? 0.f : ex2(m_ref[h][e] - mx[h][e]);
+                    if (higher) m_ref[h][e] = mx[h][e];
                     l_sum[h][e] *= alpha;
 #pragma unroll
                     for (int j = 0; j < MT; ++j) {
@@ -612,23 +612,31 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attn_kernel(const __grid
                         if (p.lse && gq == 0 && row < rows)
                             p.lse[(int64_t)at.b * p.Hq + h0 + row] = l_sum[h][e] == 0.f ? -INFINITY : (m_ref[h][e] + log2f(l_sum[h][e])) * LN2;
                     }
-                    T *out = reinterpret_cast<T *>(p.o) + (int64_t)at.b * p.o_sb + (int64_t)(h0 + h * 8 + gq) * p.o_sh;
+                    // a head's two neighbouring channels, for one store; all lanes take part in the transposes
+                    uint32_t y[MT][2];
 #pragma unroll
                     for (int j = 0; j < MT; ++j)
 #pragma unroll
-                        for (int r = 0; r < 2; ++r) {
-                            // a head's two neighbouring channels, for one store
-                            const uint32_t y = transposed(attn::Mma<T>::pack(o[j][h][r * 2] * inv[0], o[j][h][r * 2 + 1] * inv[1]));
-                            const int c = j * 16 + r * 8 + tq * 2;
-                            if (h * 8 + gq >= rows) continue;
-                            if constexpr (VEC) {
-                                if (c < p.d) *reinterpret_cast<uint32_t *>(out + c) = y;
-                            } else {
-                                const uint16_t y0 = (uint16_t)y, y1 = (uint16_t)(y >> 16);
-                                if (c < p.d) reinterpret_cast<uint16_t *>(out)[c] = y0;
-                                if (c + 1 < p.d) reinterpret_cast<uint16_t *>(out)[c + 1] = y1;
+                        for (int r = 0; r < 2; ++r)
+                            y[j][r] = transposed(attn::Mma<T>::pack(o[j][h][r * 2] * inv[0], o[j][h][r * 2 + 1] * inv[1]));
+                    __syncwarp();
+                    if (h * 8 + gq < rows) {
+                        T *out = reinterpret_cast<T *>(p.o) + (int64_t)at.b * p.o_sb + (int64_t)(h0 + h * 8 + gq) * p.o_sh;
+#pragma unroll
+                        for (int j = 0; j < MT; ++j)
+#pragma unroll
+                            for (int r = 0; r < 2; ++r) {
+                                const int c = j * 16 + r * 8 + tq * 2;
+                                if constexpr (VEC) {
+                                    if (c < p.d) *reinterpret_cast<uint32_t *>(out + c) = y[j][r];
+                                } else {
+                                    const uint16_t y0 = (uint16_t)y[j][r], y1 = (uint16_t)(y[j][r] >> 16);
+                                    if (c < p.d) reinterpret_cast<uint16_t *>(out)[c] = y0;
+                                    if (c + 1 < p.d) reinterpret_cast<uint16_t *>(out)[c + 1] = y1;
+                                }
                             }
-                        }
+                    }
+                    __syncwarp();
                 }
             } else if (!merge) {
                 float *part = part_of(p, warps, D, me, whole ? 1 : 0);
