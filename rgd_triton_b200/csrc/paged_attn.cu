@@ -70,7 +70,11 @@ __device__ __forceinline__ int live_length(const AttnParams &p, int b, bool repo
 // (16 sequences of 8000 keys, 2 cache heads with 16 heads of 128 each: 45 us, 43 with heads as rows).
 //
 // Weights are split into two numbers of the cache's type (hi + lo): rounded to one, they would cost as much accuracy
-// as the output's own rounding, and the matrix pipe idles anyway.
+// as the output's own rounding, and the matrix pipe idles anyway.  Two bf16 numbers hold a weight to 2^-18 of itself,
+// which is noise: it averages out over the keys.  fp16 ends at 2^-24, where it would drop all weights below 2^-25 of the
+// largest while the row sum counts them: 30 thousand keys 17 nats below one other came out 44 % off.  So fp16 weights
+// are multiplied by 2^15 first, and the output by 2^-15 when it leaves the registers (both exact): they are held to 2^-22
+// of themselves and 2^-40 of the largest.
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int WARPS = 4, THREADS = WARPS * 32, ROWS = 16, STAGES = 3, CTAS_PER_SM = 2;
 // In tiles: what a unit's queries and output cost, and the least run of a warp.  us for 64 sequences of 16 to 8192 keys
@@ -80,6 +84,9 @@ constexpr int UNIT_COST = 2, MIN_COST = 3;
 static_assert(MIN_COST > UNIT_COST, "a run that begins a unit has its first tile");
 
 __host__ __device__ constexpr int tile_keys(int D) { return D > 64 ? 16 : 32; }      // 8 KB of keys and values
+
+template <typename T> struct WeightScale { static constexpr float UP = 1.f, DOWN = 1.f; };
+template <> struct WeightScale<__half> { static constexpr float UP = 32768.f, DOWN = 1.f / UP; };      // a weight is at most 1, 65504 the largest fp16
 
 constexpr int NEAR = 256;               // distances whose bucket is looked up
 
@@ -423,7 +430,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attn_kernel(const __grid
 #pragma unroll
                 for (int j = 0; j < MT; ++j)
 #pragma unroll
-                    for (int r = 0; r < 2; ++r) to_o[row * D + j * 16 + r * 8 + gq] = o[j][h][r * 2 + e];
+                    for (int r = 0; r < 2; ++r) to_o[row * D + j * 16 + r * 8 + gq] = o[j][h][r * 2 + e] * WeightScale<T>::DOWN;
             }
     };
 
@@ -579,6 +586,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attn_kernel(const __grid
                     for (int e = 0; e < 2; ++e) {
                         pr[e] = ex2(s[t][h][r * 2 + e] - (m_ref[h][e] == -INFINITY ? 0.f : m_ref[h][e]));
                         l_sum[h][e] += pr[e];
+                        pr[e] *= WeightScale<T>::UP;
                         rest[e] = pr[e] - round_to<T>(pr[e]);
                     }
                     hi[h][r] = transposed(attn::Mma<T>::pack(pr[0], pr[1]));
@@ -608,7 +616,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attn_kernel(const __grid
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         const int row = h * 8 + tq * 2 + e;
-                        inv[e] = l_sum[h][e] == 0.f ? 0.f : 1.f / l_sum[h][e];
+                        inv[e] = l_sum[h][e] == 0.f ? 0.f : WeightScale<T>::DOWN / l_sum[h][e];
                         if (p.lse && gq == 0 && row < rows)
                             p.lse[(int64_t)at.b * p.Hq + h0 + row] = l_sum[h][e] == 0.f ? -INFINITY : (m_ref[h][e] + log2f(l_sum[h][e])) * LN2;
                     }

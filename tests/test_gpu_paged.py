@@ -500,3 +500,36 @@ def test_inference_mode_and_empty_calls():
     nothing = F_.paged_attention_func(q, kc[:0], vc[:0], table[:, :0], torch.zeros_like(n))
     assert (nothing == 0).all()
     assert _lib.load().rgd_device_status() == 0
+
+
+@pytest.mark.parametrize("Hq,Hk,d", [(1, 1, 64), (16, 1, 64), (6, 2, 128), (3, 1, 40)])
+@pytest.mark.parametrize("B,n", [(1200, 8192), (2, 800)])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_many_keys_far_below_one_count(Hq, Hk, d, B, n, dtype):
+    """One key with a value of 0, and all the others with one score far below it: the output is their weight alone.  With
+    a run of one warp as long as a sequence (more units than warps), and with few keys (a CTA per unit).
+
+    The products are exact (one channel).  A score in base 2 is scale * log2(e) (half a step of fp32) times that, rounded:
+    off by 2^-23 of itself, the base-2 exponential by 2^-22, the two 16-bit numbers by 2^-18 of the weight (bf16) or
+    2^-22 and 2^-40 of the largest (fp16).  Two sums for 16 keys, each off by at most a step: 2 n / 16 * 2^-23; the row
+    sum, in 8 lanes: n / 8 * 2^-24.  The output's rounding at the end."""
+    dt, page = DTYPES[dtype], 64
+    pages = -(-n // page)
+    v = torch.rand(pages, page, Hk, d, generator=gen(23)).to(dt)
+    v[0, 0] = 0
+    table = torch.arange(pages, dtype=torch.int32).cuda()[None].expand(B, -1)       # all sequences read the same pages
+    lengths = torch.full((B,), n, dtype=torch.int32, device="cuda")
+    q = torch.zeros(B, 1, Hq, d, dtype=dt)
+    q[..., 0] = 8
+    for gap in (9.0, 12.0, 15.0, 17.0, 17.375, 19.0):       # exact in both types
+        k = torch.zeros(pages, page, Hk, d, dtype=dt)
+        k[0, 0, :, 0] = gap
+        o, lse = F_.paged_attention_func(q.cuda(), k.cuda(), v.cuda(), table, lengths, softmax_scale=0.125, return_lse=True)
+        weight = math.exp(-gap)
+        total = 1 + (n - 1) * weight
+        want = (v.flatten(0, 1)[:n].double().sum(0) * weight / total).repeat_interleave(Hq // Hk, 0)
+        split = 2.0 ** -18 if dtype == "bf16" else 2.0 ** -22 + 2.0 ** -40 / weight
+        off = 2.0 ** -23 * gap / math.log(2) + 2.0 ** -22 + split + n / 8 * 2.0 ** -23 + n / 8 * 2.0 ** -24
+        slack = (2 * off + P.HALF_STEP[dt]) * want + P.TINY[dt]
+        assert ((o[:, 0].double().cpu() - want).abs() <= slack).all(), f"gap {gap}: {((o[:, 0].double().cpu() - want).abs() / want).max():.2e}"
+        assert (lse.double().cpu() - (gap + math.log(total))).abs().max() <= 2 * off + 2.0 ** -22 * gap
