@@ -533,3 +533,27 @@ def test_many_keys_far_below_one_count(Hq, Hk, d, B, n, dtype):
         slack = (2 * off + P.HALF_STEP[dt]) * want + P.TINY[dt]
         assert ((o[:, 0].double().cpu() - want).abs() <= slack).all(), f"gap {gap}: {((o[:, 0].double().cpu() - want).abs() / want).max():.2e}"
         assert (lse.double().cpu() - (gap + math.log(total))).abs().max() <= 2 * off + 2.0 ** -22 * gap
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_sums_over_a_long_run_do_not_drift(d):
+    """131 thousand keys in one warp's run (more units than warps; all sequences read the same pages), values of one sign.
+
+    Each output: its rounding (half a step), the weights (as in the plain form's bound) and two sums, of the products and of
+    the weights, of n / 16 and n / 8 terms that are rounded each (half a step of fp32).  Together: these errors have either
+    sign, and the mean over the outputs, of which the rounding to fp16 is by far the largest and uniform in its step, stays
+    within six times half a step / sqrt(3 outputs)."""
+    n, page, Hk, B, dt = 131072, 64, 512 // d, 1 + 1200 * d // 512, torch.float16
+    g = gen(d)
+    k, v = randn(g, n // page, page, Hk, d, dtype=dt).cuda(), torch.rand(n // page, page, Hk, d, generator=g).to(dt).cuda()
+    q = randn(g, 1, 1, Hk, d, dtype=dt).cuda()
+    table = torch.arange(n // page, dtype=torch.int32, device="cuda")[None].expand(B, -1)
+    lengths = torch.full((B,), n, dtype=torch.int32, device="cuda")
+    o = F_.paged_attention_func(q.expand(B, 1, Hk, d), k, v, table, lengths)[:, 0].double()
+    kd, vd, qd = k.flatten(0, 1).double(), v.flatten(0, 1).double(), q[0, 0].double()
+    want = torch.einsum("hk,khd->hd", torch.softmax(torch.einsum("hd,khd->hk", qd, kd) * d ** -0.5, -1), vd)
+    e = (d + 8) * 2.0 ** -24 * (torch.einsum("hd,khd->hk", qd.abs(), kd.abs()) * d ** -0.5).max()
+    weights = 2 * (2 * e + 2.0 ** -20) + 2.0 ** -18
+    off = o / want - 1
+    assert off.abs().max() <= P.HALF_STEP[dt] + weights + 3 * n / 16 * 2.0 ** -24
+    assert off.mean((1, 2)).abs().max() <= 6 * P.HALF_STEP[dt] / math.sqrt(3 * Hk * d) + weights
