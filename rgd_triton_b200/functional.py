@@ -139,10 +139,18 @@ def _bind_host(t):
     return _HOST
 
 
+def _has_tangent(*tensors) -> bool:
+    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def _needs_grad(*tensors) -> bool:
-    """Whether autograd has to record this call.  When it does not, the entry
+    """Whether autograd has to see this call.  When it does not, the entry
     points run the forward directly instead of through autograd.Function, whose
-    bookkeeping costs more host time than a small operator's whole launch."""
+    bookkeeping costs more host time than a small operator's whole launch.  A
+    forward-mode tangent counts, with gradients switched off too: the functions
+    carry it on or, without a jvp, refuse it."""
+    if _has_tangent(*tensors):
+        return True
     if not torch.is_grad_enabled():
         return False
     for t in tensors:
@@ -1151,17 +1159,22 @@ def _relbias_backward(dbias, buckets, wdtype, bidirectional, max_distance, offse
 
 class RelativePositionBiasFunc(torch.autograd.Function):
     """weight[bucket(j - i - offset)] as a (1, nheads, seqlen_q, seqlen_k) bias; the gradient sums the bias's over
-    each bucket's positions, in a fixed order."""
+    each bucket's positions, in a fixed order.  Linear in weight: a tangent is the bias of the weight's tangent."""
 
     @staticmethod
     def forward(ctx, weight, seqlen_q, seqlen_k, bidirectional, max_distance, offset, dtype):
         ctx.args = weight.shape[0], weight.dtype, bidirectional, max_distance, offset
+        ctx.forward_args = seqlen_q, seqlen_k, bidirectional, max_distance, offset, dtype
         return _relbias_forward(weight, seqlen_q, seqlen_k, bidirectional, max_distance, offset, dtype)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dbias):
         return _relbias_backward(dbias, *ctx.args), None, None, None, None, None, None
+
+    @staticmethod
+    def jvp(ctx, weight, *_):
+        return _relbias_forward(weight, *ctx.forward_args)
 
 
 def relative_position_bias_fn(weight, seqlen_q, seqlen_k, bidirectional=True, max_distance=128, offset=0, dtype=None):
@@ -1218,9 +1231,8 @@ def _paged_struct(k_cache, v_cache, page_table, lengths) -> Paged:
 
 
 def _refuse_grad(what: str, *tensors) -> None:
+    _require(not _has_tangent(*tensors), f"{what} has no forward-mode derivative")
     _require(not _needs_grad(*tensors), f"{what} has no backward pass: call it under torch.no_grad()")
-    if forward_ad._current_level >= 0:
-        _require(all(t is None or forward_ad.unpack_dual(t).tangent is None for t in tensors), f"{what} has no forward-mode derivative")
 
 
 def _written(*caches) -> None:

@@ -199,3 +199,34 @@ def test_one_tensor_for_both_caches_is_refused_and_left_alone():
     with pytest.raises(AssertionError, match="share memory"):
         F_.paged_cache_append_fn(k, v, kc, kc, table, lengths)
     assert torch.equal(kc, before)
+
+
+def test_a_tangent_of_the_bias_weights_is_the_bias_of_the_tangent():
+    """With and without a gradient beside it."""
+    w, t = (randn(gen(i), 32, 5, dtype=torch.bfloat16).cuda() for i in (5, 6))
+    want = F_.relative_position_bias_fn(t, 40, 61, dtype=torch.float32)
+    for wants_grad in (False, True):
+        for grad_mode in (False, True):
+            with fw.dual_level(), torch.set_grad_enabled(grad_mode):
+                leaf = w.clone().requires_grad_(wants_grad)
+                out = F_.relative_position_bias_fn(fw.make_dual(leaf, t), 40, 61, dtype=torch.float32)
+                value, tangent = fw.unpack_dual(out)
+                assert torch.equal(value, F_.relative_position_bias_fn(w, 40, 61, dtype=torch.float32)) and torch.equal(tangent, want)
+            if wants_grad and grad_mode:
+                dw, = torch.autograd.grad(out, leaf, torch.ones_like(value))
+                assert torch.equal(dw, torch.autograd.grad(F_.relative_position_bias_fn(leaf, 40, 61, dtype=torch.float32), leaf, torch.ones_like(value))[0])
+
+
+@pytest.mark.parametrize("op", ["l2", "rms", "headln", "rope", "lnrope", "attn"])
+@pytest.mark.parametrize("grad_mode", [False, True])
+def test_a_tangent_of_an_input_without_gradient_is_refused(op, grad_mode):
+    x = randn(gen(7), 2, 9, 64).cuda()
+    q, k = (randn(gen(i), 2, 24, 3, 64, dtype=torch.float16).cuda() for i in (8, 9))
+    pos = rotary_table(64, 32, torch.float16).cuda()
+    call, t = {"l2": (ops.L2Normalize(), x), "rms": (ops.FusedRMSNorm(64).cuda(), x), "headln": (lambda a: ops.FusedHeadLayerNorm()(a, k, False), q),
+               "rope": (lambda a: ops.RoPE()(a, k, pos, 20, False), q), "lnrope": (lambda a: ops.FusedLNRoPE()(a, k, pos, (20, 24), False), q),
+               "attn": (lambda a: ops.FlashAttention()(a, k, k), q)}[op]
+    with fw.dual_level(), torch.set_grad_enabled(grad_mode):
+        call(t)
+        with pytest.raises(RuntimeError):
+            call(fw.make_dual(t, torch.ones_like(t)))
