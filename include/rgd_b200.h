@@ -438,8 +438,11 @@ int rgd_paged_slot(const rgd_paged *cache, int64_t row, int64_t position,
  * `query` (B, Hq, N, d; may be NULL) into query_out; rows of query past counts[b]
  * are copied.  fp32 arithmetic, one rounding.  A token whose position is not in
  * the cache or not below P is not written.  Two tokens of one call that map to
- * the same slot leave either's values there, channel by channel.  dtype RGD_F16
- * / RGD_BF16, pos_dtype any, d <= 128, B * N <= 2^30, max_pages * page_size below
+ * the same slot leave either's values there, channel by channel.  The slots of
+ * k and of v must not share memory with one another nor with the inputs: k == v
+ * is refused (RGD_E_INVALID), other overlaps are the caller's to avoid (keys and
+ * values side by side in one tensor are fine).  dtype RGD_F16 / RGD_BF16,
+ * pos_dtype any, d <= 128, B * N <= 2^30, max_pages * page_size below
  * 2^31 - 1024. */
 int rgd_paged_append(const rgd_heads *key, const rgd_heads *value,
                      const rgd_heads *query, const rgd_heads *query_out,

@@ -297,6 +297,7 @@ extern "C" int rgd_paged_append(const rgd_heads *key, const rgd_heads *value, co
     if (!query) Hq = 0;
     if (B == 0 || N == 0 || d == 0 || (Hq == 0 && Hkv == 0)) return RGD_OK;
     if ((Hkv > 0 && (!key->ptr || !value->ptr)) || (Hq > 0 && (!query->ptr || !query_out->ptr))) return RGD_E_NULL;
+    if (Hkv > 0 && cache->num_pages > 0 && cache->k == cache->v) return RGD_E_INVALID;      // keys and values in the same slots
 
     paged::AppendParams p{};
     p.view = paged::make_view(*cache);

@@ -1307,7 +1307,8 @@ def paged_cache_append_fn(key, value, k_cache, v_cache, page_table, lengths, pos
     Returns the rotated query, or None without one.  lengths is not changed.  Nothing is read back from the device:
     a token whose position has no page, or no row in pos_emb, is left out, and
     ``rgd_triton_b200._lib.load().rgd_device_status()`` reports it.  No two tokens of a call may map to the same slot.
-    No backward pass."""
+    The caches must not share memory with one another (one tensor for both is refused; keys and values side by side in one
+    tensor are fine) nor with the tokens.  No backward pass."""
     if _tracing():
         out = torch.ops.rgd_b200.paged_append(key, value, k_cache, v_cache, page_table, lengths, pos_emb, query, counts)
         return None if query is None else out

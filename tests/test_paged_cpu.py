@@ -204,3 +204,13 @@ def test_c_abi_refuses_negative_gradient_strides_and_too_many_sequences():
     cache = _paged(torch.zeros(1, 0, dtype=torch.int32))                # no page: nothing else bounds the sequences
     assert lib.rgd_paged_attn(h, C.byref(cache), None, h, None, (1 << 30) + 1, 1, 1, 64, 1.0, _lib.RGD_F16, None, 0, None) == _lib.RGD_E_SIZE
     assert lib.rgd_paged_attn_workspace_bytes((1 << 30) + 1, 1, 1, 64, 0, 16) == _lib.RGD_E_SIZE
+
+
+def test_c_abi_refuses_one_cache_for_keys_and_values():
+    lib = _lib.load()
+    h = C.byref(_lib.Heads(16, 8, 8, 8))
+    table = torch.zeros(1, 4, dtype=torch.int32)
+    append = lambda cache, N=1, Hkv=2: lib.rgd_paged_append(h, h, None, None, C.byref(cache), None, None, 0, 0, 0, 0, 1, N, 0, Hkv, 64,
+                                                            _lib.RGD_F16, _lib.RGD_F16, None)
+    assert append(_paged(table, k=16)) == _lib.RGD_E_INVALID
+    assert append(_paged(table, k=16), N=0) == 0 and append(_paged(table, k=16), Hkv=0) == 0        # nothing to write
