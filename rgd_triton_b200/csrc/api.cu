@@ -43,26 +43,24 @@ struct LaunchKeyHash {
     }
 };
 std::mutex g_launch_memo_mutex;
-std::unordered_map<LaunchKey, int, LaunchKeyHash> g_smem_memo, g_occ_memo;
+std::unordered_map<LaunchKey, size_t, LaunchKeyHash> g_smem_memo;       // most bytes asked for
+std::unordered_map<LaunchKey, int, LaunchKeyHash> g_occ_memo;
 }  // namespace
 
 int ensure_dyn_smem(const void *kernel, size_t bytes) {
     int dev = 0;
     if (cudaError_t e = cudaGetDevice(&dev); e != cudaSuccess) return cuda_status(e);
-    const LaunchKey key{dev, kernel, (uint64_t)bytes, 0};
-    {
-        std::lock_guard<std::mutex> lock(g_launch_memo_mutex);
-        auto it = g_smem_memo.find(key);
-        if (it != g_smem_memo.end()) return it->second;
-    }
+    const LaunchKey key{dev, kernel, 0, 0};
+    std::lock_guard<std::mutex> lock(g_launch_memo_mutex);      // over the driver call too: limits are set in the order of the memo
+    auto it = g_smem_memo.find(key);
+    if (it != g_smem_memo.end() && it->second >= bytes) return RGD_OK;
     const int rc = cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
     if (rc != RGD_OK) {
         (void)cudaGetLastError();
         return rc;                      // not memoised: the next call asks the driver again
     }
-    std::lock_guard<std::mutex> lock(g_launch_memo_mutex);
-    g_smem_memo[key] = rc;
-    return rc;
+    g_smem_memo[key] = bytes;
+    return RGD_OK;
 }
 
 int cached_occupancy(const void *kernel, int threads, size_t smem) {

@@ -16,8 +16,8 @@ namespace rgd {
 void count_launch();                    // defined in api.cu
 int  check_launch();                    // cudaGetLastError -> status code
 int  num_sms();                         // SM count of the current device (cached)
-// Opt a kernel in to `bytes` of dynamic shared memory.  The driver call is made once per
-// (device, kernel, size); later launches only look the answer up.
+// Opt a kernel in to `bytes` of dynamic shared memory.  The driver call is made only where a kernel asks for more than
+// it has had on this device: each call sets the limit anew, so one for less would take the larger one back.
 int  ensure_dyn_smem(const void *kernel, size_t bytes);
 // cudaOccupancyMaxActiveBlocksPerMultiprocessor, memoised per (device, kernel, threads,
 // shared memory).  Never returns less than 1.
