@@ -557,3 +557,35 @@ def test_sums_over_a_long_run_do_not_drift(d):
     off = o / want - 1
     assert off.abs().max() <= P.HALF_STEP[dt] + weights + 3 * n / 16 * 2.0 ** -24
     assert off.mean((1, 2)).abs().max() <= 6 * P.HALF_STEP[dt] / math.sqrt(3 * Hk * d) + weights
+
+
+@pytest.mark.parametrize("layout", ["tokens", "heads"])
+def test_attention_of_a_padded_prompt_over_its_gathered_keys(layout):
+    """A padded batch of prompts with grouped heads: the append rotates the query, the rotated keys are gathered from the
+    pages, and the causal attention of the real rows is that of the rotated tokens.  FlashAttention rounds its weights
+    and its output to bf16: two half steps of the largest value, twice that for the second product's own rounding."""
+    g = gen(24)
+    B, n, heads, heads_k, d, page, dt = 3, 37, 8, 2, 64, 16, torch.bfloat16
+    counts = torch.tensor([37, 5, 20], dtype=torch.int32)
+    table, pages = _table(g, counts.tolist(), page)
+    kc, vc = (_gpu(t) for t in _pool(g, pages, page, heads_k, d, dt, layout))
+    key, value, query = (randn(g, B, n, h, d, dtype=dt) for h in (heads_k, heads_k, heads))
+    pos = rotary_table(n, d, torch.float32)
+    lengths, page_table = torch.zeros(B, dtype=torch.int32).cuda(), table.cuda()
+    _, _, rotated = P.append(key, value, torch.zeros(pages, page, heads_k, d), torch.zeros(pages, page, heads_k, d), table, torch.zeros(B, dtype=torch.int32), pos, query, counts)[0]
+    q = F_.paged_cache_append_fn(key.cuda(), value.cuda(), kc, vc, page_table, lengths, pos.cuda(), query.cuda(), counts.cuda())
+    used = page_table[:, :(n + page - 1) // page].long().clamp(min=0)
+    k = kc[used].flatten(1, 2)[:, :n]
+    share = heads // heads_k
+    o = F_.flash_attn_func(q, k.repeat_interleave(share, 2), value.cuda().repeat_interleave(share, 2), causal=True).double().cpu()
+    sin, cos = pos.double()
+    for b in range(B):
+        m = int(counts[b])
+        x = key[b, :m].double()
+        kr = torch.stack([x[..., 0::2] * cos[:m, None, 0::2] - x[..., 1::2] * sin[:m, None, 0::2],
+                          x[..., 1::2] * cos[:m, None, 1::2] + x[..., 0::2] * sin[:m, None, 1::2]], -1).flatten(-2).to(dt).double()
+        kr, v = kr.repeat_interleave(share, 1), value[b, :m].double().repeat_interleave(share, 1)
+        s = torch.einsum("ihd,jhd->hij", rotated[b, :m].to(dt).double(), kr) * d ** -0.5
+        s = s.masked_fill(torch.ones(m, m, dtype=torch.bool).triu(1), -math.inf)
+        want = torch.einsum("hij,jhd->ihd", s.softmax(-1), v)
+        assert (o[b, :m] - want).abs().max() <= 4 * 2.0 ** -8 * v.abs().max()
