@@ -462,7 +462,9 @@ int64_t rgd_paged_attn_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv,
  * d) views; query head h reads cache head h / (Hq / Hkv).  `bias` (NULL: none)
  * adds weight[bucket(lengths[b] - 1 - j), h].  lse (NULL or fp32 [B, Hq]):
  * log-sum-exp.  A sequence of length 0 gets zeros and lse -inf; so does one
- * without a usable page.  Keys of pages out of range are left out.  dtype
+ * without a usable page.  Keys of pages out of range are left out.  An infinity
+ * or NaN in a live key or value is not masked: an output that it reaches is
+ * infinite or NaN.  dtype
  * RGD_F16 / RGD_BF16, d <= 128, Hq a multiple of Hkv, B <= 2^30, B * Hkv *
  * ceil(Hq / Hkv / 16) * (max_pages * page_size / 16 + 3) below 2^31.  The order
  * of all sums depends on the lengths, max_pages, page_size and the device, not on

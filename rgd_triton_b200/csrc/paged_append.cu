@@ -82,7 +82,8 @@ template <> __device__ __forceinline__ float2 unpack<__nv_bfloat16>(uint32_t w) 
 // looked up once for the CTA, two dependent reads (length; table entry and angles) during which the first tokens are on
 // their way; the loop is then read, turn, write.  [4, 4096, 16, 128] bf16 keys, values and queries (411 MB): 73 us, 86 %
 // of the copy rate, bound by instruction issue (two thirds of the slots busy) and the look-ups.  With every thread
-// looking up its own tokens it took 160-200 us.  Four CTAs an SM: 74 us at five, and ragged sequences 6.6 us for 6.0.
+// looking up its own tokens it took 160-200 us.  Four CTAs an SM: 74 us at five, and ragged sequences 6.6 us for 6.0.  Pairs (VE = 2) are what odd views cost: [4, 2048, 16, 128] 142 us one
+// element off 16 bytes, 39 us on them.
 template <typename T, int VE>
 __global__ void __launch_bounds__(APPEND_THREADS, 4) append_kernel(const __grid_constant__ AppendParams p) {
     using V = Vec<uint32_t, VE / 2>;            // pairs of channels

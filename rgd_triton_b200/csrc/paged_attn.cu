@@ -176,7 +176,8 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
     return y;
 }
 
-// HT: column tiles of 8 query heads.
+// HT: column tiles of 8 query heads.  VEC: rows of 16-byte words; without it every element is a guarded 2-byte load that the
+// warp waits for (16 sequences of 4000 keys, 32 / 8 heads of 128: 49 us, one element off 575, heads of 100 channels 430).
 template <typename T, int D, bool VEC, bool BIAS, int HT>
 __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attn_kernel(const __grid_constant__ AttnParams p) {
     using S = Smem<T, D>;
@@ -866,12 +867,18 @@ bool too_large(int64_t B, int64_t units, int64_t max_keys, int D) {
 
 // How the tiles are spread.  Few units of few keys (by what the table has room for; the lengths are not known here): a CTA
 // per unit, which needs no schedule, no workspace and no second launch.  Others: what the SMs hold at once, and no more
-// CTAs than there can be runs.  us of GPU time in equal runs / a CTA per unit, at 8, 16, 24, 32, 48 tiles:
-//   16 units, head_dim 64     14.3 / 10.2   14.3 / 12.3   14.3 / 14.3   14.3 / 16.5   14.3 / 22.5
-//   64 units, head_dim 128    14.3 / 10.2   14.3 / 12.3   16.4 / 14.3   16.4 / 18.4   18.4 / 22.5
-//   256 units, head_dim 64    16.4 / 12.3   18.4 / 14.3   22.5 / 18.4   24.6 / 20.5   28.7 / 26.6
-//   512 units, head_dim 128   20.5 / 18.4   24.6 / 24.6   28.7 / 28.7   34.8 / 34.8   44.9 / 45.1
-//   2048 units, head_dim 128  36.9 / 45.1   57.3 / 67.6   77.8 / 90.1   98.3 / 109    139 / 143
+// CTAs than there can be runs.  us of a call, many in a row over different caches, a CTA per unit / equal runs, all
+// sequences as long as the table or of 16 keys up to that (even over the logarithm), at 8, 16, 24, 32, 48 tiles:
+//   16 units, head_dim 64       5.1 / 8.7     7.2 / 9.4     9.9 / 10.0   12.4 / 9.4    17.5 / 10.3
+//   64 units, head_dim 128      5.9 / 9.3     8.4 / 10.6   11.0 / 11.5   13.5 / 11.3   18.3 / 12.5
+//   148 units, head_dim 128     6.1 / 10.2    8.5 / 11.6   11.0 / 13.3   13.4 / 15.5   18.1 / 18.6
+//     mixed lengths             5.4 / 9.8     7.7 / 11.1   10.4 / 11.3   12.7 / 10.9   17.1 / 11.4
+//   256 units, head_dim 64      7.0 / 10.8    9.7 / 12.8   13.3 / 16.5   16.3 / 19.2   22.2 / 24.7
+//     mixed lengths             5.6 / 9.5     7.7 / 9.6    11.2 / 11.4   13.3 / 11.3   18.5 / 12.8
+//   512 units, head_dim 128    13.2 / 14.9   18.8 / 19.8   25.1 / 25.7   30.3 / 31.1   40.8 / 41.4
+//     mixed lengths            10.3 / 11.4   12.6 / 12.7   16.7 / 15.4   19.6 / 15.2   18.9 / 16.8
+// Few units and mixed lengths are even at about 25 tiles whatever the units, so one limit serves all; many units of one
+// length would gain 2-3 us from a CTA each up to 50 tiles, but no call says that its lengths are alike.
 constexpr int DIRECT_TILES = 28;
 struct Plan {
     bool direct;

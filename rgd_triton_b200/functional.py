@@ -1298,7 +1298,8 @@ def paged_cache_append_fn(key, value, k_cache, v_cache, page_table, lengths, pos
 
     key, value: (batch, n, nheads_k, headdim), n new tokens of each sequence; k_cache, v_cache: (pages, page_size,
     nheads_k, headdim), written in place, any strides with a unit channel stride (a cache kept head by head is passed
-    as its transpose(1, 2)); page_table: (batch, max_pages) int32, the page of each page_size positions of a sequence;
+    as its transpose(1, 2); views that 16-byte accesses do not reach, by their start, a stride or a head dim that is not a
+    multiple of 8, cost several times as much here and in the attention); page_table: (batch, max_pages) int32, the page of each page_size positions of a sequence;
     lengths: (batch,) int32, the tokens that each sequence holds so far.  Token i of sequence b goes to position
     lengths[b] + i.  ``counts``: (batch,) int32, only the first counts[b] tokens are new ones (default: all n).
     ``pos_emb``: [2, P, R], sin and cos as for RoPE; the first R channels of key are rotated in fp32 and rounded once.
@@ -1367,7 +1368,8 @@ def paged_attention_func(q, k_cache, v_cache, page_table, lengths, softmax_scale
     ``return_lse`` the (batch, nheads) log-sum-exp.
 
     Nothing is read back from the device: keys of pages outside the pool are left out, a length past the table's pages
-    is cut there, and ``rgd_triton_b200._lib.load().rgd_device_status()`` reports both.  No backward pass."""
+    is cut there, and ``rgd_triton_b200._lib.load().rgd_device_status()`` reports both.  What lies past a sequence is not used; an
+    infinity or NaN in its own keys and values is not masked: an output that it reaches is infinite or NaN.  No backward pass."""
     bidirectional, max_distance = bool(bidirectional), int(max_distance)
     if _tracing():
         o, lse = torch.ops.rgd_b200.paged_attn(q, k_cache, v_cache, page_table, lengths, softmax_scale, rel_weight, bidirectional, max_distance)
